@@ -74,7 +74,7 @@ def draw(rng):
     k = _log(rng, 16, 8192)
     n = _log(rng, 1, 8192)
     return {"op": op, "m": _log(rng, 1, max(1, min(16384, 250_000_000_000 // (n * k)))), "n": n, "k": k,
-            "out": rng.choice(["bf16", "fp32", "fp16"]), "bias": flag()}
+            "out": rng.choice(["bf16", "fp16"]), "bias": flag()}
 
 
 def work(case):
