@@ -17,7 +17,7 @@ LIB_PATH = os.environ.get("DSSM_LIB_PATH", LIB_PATH)
 
 DSSM_ABI_VERSION = 2
 DSSM_MAX_LAYERS = 8
-DSSM_F32, DSSM_BF16, DSSM_I32 = 0, 1, 2
+DSSM_F32, DSSM_BF16, DSSM_I32, DSSM_F16 = 0, 1, 2, 3
 DSSM_ACT_NONE, DSSM_ACT_RELU = 0, 1
 (BUF_LOSS, BUF_COS_SIM_RAW, BUF_COS_SIM, BUF_PROB, BUF_QUERY_NORM, BUF_EMBED, BUF_Z,
  BUF_BATCH_MEAN, BUF_BATCH_VAR, BUF_DZ) = range(10)
@@ -63,6 +63,7 @@ class dssm_segment(C.Structure):
 
 
 _P = C.c_void_p
+_L = C.c_int64
 _SIGS = {
     "dssm_abi_version": (C.c_int, []),
     "dssm_last_error": (C.c_char_p, []),
@@ -227,6 +228,23 @@ _SIGS = {
     "dssm_plan_peer_exchange": (C.c_int, [_P, C.c_int, _P]),
     "dssm_plan_peer_status": (C.c_int, [_P, _P]),
     "dssm_plan_peer_selftest": (C.c_int, [_P, _P, _P]),
+    # sequence-tower operators (dssm_amd/seqops.py)
+    "dssm_embedding_lookup": (C.c_int, [_P, C.c_int, _L, _L, C.c_int, _P, C.c_int, _L, C.c_float, _P, C.c_int, _P]),
+    "dssm_embedding_grad_ws_bytes": (C.c_size_t, [_L, _L, C.c_int]),
+    "dssm_embedding_grad": (C.c_int, [_P, C.c_int, _L, _P, C.c_int, _L, _L, C.c_int, C.c_float, _P, _P, C.c_size_t, _P]),
+    "dssm_linear_recurrence_ws_bytes": (C.c_size_t, [_L, C.c_int, C.c_int, C.c_int]),
+    "dssm_linear_recurrence": (C.c_int, [_P, _L, _L, _P, _L, _L, C.c_int, _P, _P, _L, C.c_int, C.c_int, C.c_int, _P, _L,
+                                         _L, _P, _P, _P, C.c_size_t, _P]),
+    "dssm_linear_recurrence_bwd": (C.c_int, [_P, _L, _L, _P, _L, _L, C.c_int, _P, _P, _P, _L, _L, _P, _L, C.c_int,
+                                             C.c_int, C.c_int, _P, _L, _L, _P, _L, _L, _P, _P, C.c_size_t, _P]),
+    "dssm_linear_recurrence_step": (C.c_int, [_P, _L, _P, _L, C.c_int, _P, _L, _P, _L, _L, C.c_int, _P]),
+    "dssm_rms_norm": (C.c_int, [_P, _L, _P, _L, _P, _L, C.c_int, C.c_int, C.c_float, _P, _L, _P, _L, _P, _P]),
+    "dssm_rms_norm_bwd_ws_bytes": (C.c_size_t, [_L, C.c_int]),
+    "dssm_rms_norm_bwd": (C.c_int, [_P, _L, _P, _L, _P, _P, _P, _L, _L, C.c_int, C.c_int, _P, _L, _P, _P, C.c_size_t, _P]),
+    "dssm_quantize_blocks8": (C.c_int, [_P, _L, _L, C.c_int, C.c_int, _P, _P, _P]),
+    "dssm_dequantize_blocks8": (C.c_int, [_P, _P, _L, C.c_int, _P, _L, C.c_int, _P]),
+    "dssm_rms_norm_blocks8": (C.c_int, [_P, _L, _P, _L, _P, _L, C.c_int, C.c_int, C.c_float, _P, _P, _P, _L, _P, _P]),
+    "dssm_blocks8_matmul": (C.c_int, [_P, _P, _P, _P, _L, _L, _L, _P, _P, _L, C.c_int, _P]),
 }
 PEER_FLAG_BYTES = 4096  # include/dssm.h DSSM_PEER_FLAG_BYTES
 

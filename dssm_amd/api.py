@@ -17,7 +17,9 @@ Two halves:
   * `batch_normalization` (:62-88), with the ReLU fused;
   * `cosine_similarity` (Merge + Cosine_Similarity + Loss, :160-213).
 
-  Each wraps one C-ABI kernel (include/dssm.h). Torch tensors are only device storage.
+  Each wraps one C-ABI kernel (include/dssm.h). Torch tensors are only device storage. The
+  sequence-tower operators of dssm_amd/seqops.py (embedding, gated linear recurrence, RMS norm, 8-bit
+  product, each with the gradient that training needs) are part of it.
 
 Everything runs on the GPU through libdssm.so. There is no CPU fallback: a missing library raises
 at import of the model (dssm_amd._lib.load).
@@ -37,6 +39,9 @@ from . import _lib, tfckpt
 from .data import SparseTensorValue, feeds_to_csr
 from .metrics import StreamingAUC, dssm_labels
 from .model import DSSM
+from .seqops import (Blocks8, blocks8_matmul, dequantize_blocks8, embedding_grad, embedding_lookup,  # noqa: F401
+                     linear_recurrence, linear_recurrence_grad, linear_recurrence_step, quantize_blocks8, rms_norm,
+                     rms_norm_blocks8, rms_norm_grad)
 
 GAMMA = 20.0  # cos_sim scale (new_dssm.py:199)
 

@@ -1,0 +1,583 @@
+// Gated linear recurrence over sequences, its gradient, and its single-token step.
+//
+//   u_t = sigmoid(gate_t),  h_t = u_t h_{t-1} + (1 - u_t) cand_t            (TF's GRUCell convention)
+//
+// per row and channel; a step at or past the row's length carries the state and emits zero
+// (tf.nn.dynamic_rnn).  `reverse` walks the row from its last step to its first, as
+// bidirectional_dynamic_rnn's backward cell does: time is mirrored by a negative stride, and the steps past
+// the length, which the mirrored walk meets first, carry the state all the same.
+//
+// The gates do not look at the state, so steps compose: a stretch of time is the affine map
+// h -> A h + B with A = product of u.  The gradient is the same recurrence from the other end,
+//   g_t = dh_t + u_{t+1} g_{t+1},  dcand_t = (1 - u_t) g_t,  dgate_t = g_t (h_{t-1} - cand_t) u_t (1 - u_t),
+// with gamma = u g as the value that crosses from step to step (gamma -> P gamma + Q over a stretch).
+//
+// Layout: a lane owns 4 bytes of neighbouring channels of one row, a wave a piece of kPiece steps whose
+// loads are all in flight at once.  With few channels NW waves take NW consecutive pieces: each reduces
+// its piece to (A, B), they meet in LDS once, and each replays its piece from registers behind its true
+// state, so the inputs are read once.  With very few channels the time axis is also cut into segments of
+// several workgroups: one launch reduces the segments, the next folds the earlier segments' (A, B) into
+// its own start; there the inputs are read twice.
+//
+// The forward keeps the fp32 state in front of every piece (a quarter of a byte per element); the
+// backward walks a piece forward from it in registers and so needs neither h nor a forward scan.  States,
+// gates and sums are fp32 throughout.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "seq.h"
+
+namespace dssm {
+namespace seq {
+namespace {
+
+constexpr int kPiece = DSSM_RECUR_PIECE;
+
+// u = sigmoid(f) and v = 1 - u, both to fp32 accuracy: e = exp(-|f|) never overflows and neither result
+// is a difference.  exp(x) = 2^(x log2 e) with the product's rounding error and log2 e's own put back
+// (the hardware's 2^x alone would be off by |x| roundings).
+__device__ __forceinline__ void gate_uv(float f, float& u, float& v) {
+  const float x = -fabsf(f), kL = 1.44269502f, kLlo = 1.92596303e-8f;
+  const float hi = x * kL, lo = fmaf(x, kL, -hi) + x * kLlo;
+  float e = __builtin_amdgcn_exp2f(hi);
+  e = fmaf(e, lo * 0.693147182f, e);
+  e = x > -126.f * 0.69f ? e : (x == x ? 0.f : x);  // (-inf would give inf - inf)
+  const float r = __builtin_amdgcn_rcpf(1.f + e), q = e * r;
+  u = f >= 0.f ? r : q;
+  v = f >= 0.f ? q : r;
+}
+
+struct RecurArgs {
+  const void *gate, *cand, *dh;
+  int64_t gr, gt, cr, ct, dr, dt;  // row and time strides in elements
+  const int* lens;
+  const float* h0;     // [R x H], or null: zeros
+  const float* dlast;  // backward: [R x H] or null
+  void *h, *dgate, *dcand;
+  int64_t hr, ht, ogr, ogt, ocr, oct;
+  float *last, *dh0;  // forward / backward
+  float* states;      // [ceil(T / kPiece)][R x H]
+  float* sums;        // [2][S][R x H]: the segments' A and B (P and Q)
+  int64_t R;
+  int T, H, upr;  // upr: lane units per row
+  int reverse, S, L;  // segments and their steps (a multiple of NW * kPiece)
+};
+
+template <int V>
+struct Unit {  // a lane's channels
+  int64_t r, ch;  // row, first channel in [R x H]
+  int c, lo, hi;  // column; active steps [lo, hi) in walking order
+  bool in;
+};
+template <int V>
+__device__ __forceinline__ Unit<V> unit_of(const RecurArgs& a, int64_t u) {
+  Unit<V> t;
+  t.in = u < a.R * a.upr;
+  if (!t.in) u = 0;
+  t.r = u / a.upr;
+  t.c = (int)(u - t.r * a.upr) * V;
+  t.ch = t.r * a.H + t.c;
+  int len = a.T;
+  if (a.lens) len = min(max(a.lens[t.r], 0), a.T);
+  if (!t.in) len = 0;
+  t.lo = a.reverse ? a.T - len : 0;
+  t.hi = a.reverse ? a.T : len;
+  return t;
+}
+// element pointer of the unit at walking step 0, and the walking stride
+template <typename T>
+__device__ __forceinline__ T* walk(T* p, const RecurArgs& a, int64_t sr, int64_t st, int64_t r, int c) {
+  return p + r * sr + c + (a.reverse ? (int64_t)(a.T - 1) * st : 0);
+}
+
+// A piece's u and x = (1 - u) cand; steps that do not act are u = 1, x = 0.
+template <typename T, int V>
+__device__ __forceinline__ void load_piece(const T* g, int64_t gs, const T* c, int64_t cs, int q0, int lo, int hi,
+                                           float (&u)[kPiece][V], float (&x)[kPiece][V]) {
+  Pack<T, V> a[kPiece], b[kPiece];
+#pragma unroll
+  for (int i = 0; i < kPiece; ++i) {
+    const int p = q0 + i;
+    if (p >= lo && p < hi) {
+      a[i] = ldv<T, V>(g + p * gs);
+      b[i] = ldv<T, V>(c + p * cs);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPiece; ++i) {
+    const bool on = q0 + i >= lo && q0 + i < hi;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      float uu, vv;
+      gate_uv(ld1(a[i].v[k]), uu, vv);
+      u[i][k] = on ? uu : 1.f;
+      x[i][k] = on ? vv * ld1(b[i].v[k]) : 0.f;
+    }
+  }
+}
+
+// The value that enters a segment: `start` carried through the earlier segments' maps.  The waves fold a
+// share of the segments each and join through LDS.  dir > 0: segments 0 .. s - 1; dir < 0: S - 1 .. s + 1.
+template <int V, int NW>
+__device__ __forceinline__ void enter_segment(const RecurArgs& a, const Unit<V>& t, int s, int dir, float (*lds)[64][2 * V],
+                                              float (&carry)[V]) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int n = dir > 0 ? s : a.S - 1 - s, per = (n + NW - 1) / NW, k0 = min(w * per, n), k1 = min(k0 + per, n);
+  const int64_t C = a.R * a.H;
+  float A[V], B[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    A[k] = 1.f;
+    B[k] = 0.f;
+  }
+  if (t.in)
+    for (int j = k0; j < k1; ++j) {
+      const int seg = dir > 0 ? j : a.S - 1 - j;
+      const Pack<float, V> pa = ldv<float, V>(a.sums + (int64_t)seg * C + t.ch);
+      const Pack<float, V> pb = ldv<float, V>(a.sums + (int64_t)(a.S + seg) * C + t.ch);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        B[k] = fmaf(pa.v[k], B[k], pb.v[k]);
+        A[k] *= pa.v[k];
+      }
+    }
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    lds[w][lane][k] = A[k];
+    lds[w][lane][V + k] = B[k];
+  }
+  __syncthreads();
+  for (int j = 0; j < NW; ++j)
+#pragma unroll
+    for (int k = 0; k < V; ++k) carry[k] = fmaf(lds[j][lane][k], carry[k], lds[j][lane][V + k]);
+  __syncthreads();
+}
+
+// ---- forward -----------------------------------------------------------------------------------
+// SUM: only the segment's (A, B).
+template <typename T, int V, int NW, bool SUM>
+__global__ __launch_bounds__(NW * 64) void k_recur_fwd(RecurArgs a) {
+  __shared__ float lds[2][NW][64][2 * V];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  // the replay walks the segments from the last: what the summing launch read last is what caches hold
+  const int s = SUM ? (int)blockIdx.y : a.S - 1 - (int)blockIdx.y;
+  const Unit<V> t = unit_of<V>(a, (int64_t)blockIdx.x * 64 + lane);
+  const int64_t gs = a.reverse ? -a.gt : a.gt, cs = a.reverse ? -a.ct : a.ct, hs = a.reverse ? -a.ht : a.ht;
+  const T* g = walk((const T*)a.gate, a, a.gr, a.gt, t.r, t.c);
+  const T* c = walk((const T*)a.cand, a, a.cr, a.ct, t.r, t.c);
+  T* ho = walk((T*)a.h, a, a.hr, a.ht, t.r, t.c);
+  float carry[V], span[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    carry[k] = !SUM && a.h0 && t.in ? a.h0[t.ch + k] : 0.f;
+    span[k] = 1.f;
+  }
+  if constexpr (!SUM && NW > 1)
+    if (a.S > 1) enter_segment<V, NW>(a, t, s, 1, lds[0], carry);
+  const int end = min(s * a.L + a.L, a.T);
+  int buf = 0;
+  for (int p0 = s * a.L; p0 < end; p0 += NW * kPiece, buf ^= 1) {
+    const int q0 = p0 + w * kPiece;
+    float u[kPiece][V], x[kPiece][V], h[V];
+    load_piece<T, V>(g, gs, c, cs, q0, t.lo, t.hi, u, x);
+    if constexpr (NW > 1) {
+      float A[V], B[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        A[k] = 1.f;
+        B[k] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          B[k] = fmaf(u[i][k], B[k], x[i][k]);
+          A[k] *= u[i][k];
+        }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        lds[buf][w][lane][k] = A[k];
+        lds[buf][w][lane][V + k] = B[k];
+      }
+      // one barrier a round: the other half of lds is written next, and a wave that writes this half
+      // again has passed the next round's barrier, behind every wave's reads here
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NW; ++j)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          if (j == w) h[k] = carry[k];
+          carry[k] = fmaf(lds[buf][j][lane][k], carry[k], lds[buf][j][lane][V + k]);
+          if constexpr (SUM) span[k] *= lds[buf][j][lane][k];
+        }
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) h[k] = carry[k];
+    }
+    if constexpr (!SUM) {
+      if (t.in && q0 < a.T) {
+        if (a.states) {
+          Pack<float, V> st;
+#pragma unroll
+          for (int k = 0; k < V; ++k) st.v[k] = h[k];
+          stv<float, V>(a.states + (int64_t)(q0 / kPiece) * a.R * a.H + t.ch, st);
+        }
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) {
+          const int p = q0 + i;
+          const bool on = p >= t.lo && p < t.hi;
+          Pack<T, V> o;
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            h[k] = fmaf(u[i][k], h[k], x[i][k]);
+            o.v[k] = st1<T>(on ? h[k] : 0.f);
+          }
+          if (p < a.T) stv<T, V>(ho + p * hs, o);
+        }
+      }
+      if constexpr (NW == 1) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) carry[k] = h[k];
+      }
+    }
+  }
+  if (!t.in || w) return;
+  if constexpr (SUM) {
+    const int64_t C = a.R * a.H;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      a.sums[(int64_t)s * C + t.ch + k] = span[k];
+      a.sums[(int64_t)(a.S + s) * C + t.ch + k] = carry[k];
+    }
+  } else if (end == a.T) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) a.last[t.ch + k] = carry[k];
+  }
+}
+
+// ---- backward ----------------------------------------------------------------------------------
+// SUM: only the segment's (P, Q).
+template <typename T, int V, int NW, bool SUM>
+__global__ __launch_bounds__(NW * 64) void k_recur_bwd(RecurArgs a) {
+  __shared__ float lds[2][NW][64][2 * V];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int s = SUM ? a.S - 1 - (int)blockIdx.y : (int)blockIdx.y;
+  const Unit<V> t = unit_of<V>(a, (int64_t)blockIdx.x * 64 + lane);
+  const int sg = a.reverse ? -1 : 1;
+  const T* g = walk((const T*)a.gate, a, a.gr, a.gt, t.r, t.c);
+  const T* c = walk((const T*)a.cand, a, a.cr, a.ct, t.r, t.c);
+  const T* d = a.dh ? walk((const T*)a.dh, a, a.dr, a.dt, t.r, t.c) : nullptr;
+  T* og = walk((T*)a.dgate, a, a.ogr, a.ogt, t.r, t.c);
+  T* oc = walk((T*)a.dcand, a, a.ocr, a.oct, t.r, t.c);
+  float carry[V], span[V];  // carry: gamma, the gradient that reaches the state behind the current stretch
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    carry[k] = !SUM && a.dlast && t.in ? a.dlast[t.ch + k] : 0.f;
+    span[k] = 1.f;
+  }
+  if constexpr (!SUM && NW > 1)
+    if (a.S > 1) enter_segment<V, NW>(a, t, s, -1, lds[0], carry);
+  const int begin = s * a.L, end = min(begin + a.L, a.T);
+  int buf = 0;
+  for (int p0 = begin + (end - begin - 1) / (NW * kPiece) * (NW * kPiece); p0 >= begin; p0 -= NW * kPiece, buf ^= 1) {
+    const int q0 = p0 + w * kPiece;
+    Pack<T, V> ra[kPiece], rb[kPiece], rd[kPiece];
+    float hp[V];
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) {
+      const int p = q0 + i;
+      if (p >= t.lo && p < t.hi) {
+        ra[i] = ldv<T, V>(g + sg * p * a.gt);
+        if constexpr (!SUM) rb[i] = ldv<T, V>(c + sg * p * a.ct);
+        if (d) rd[i] = ldv<T, V>(d + sg * p * a.dt);
+      }
+    }
+    if constexpr (!SUM) {
+      Pack<float, V> st;
+#pragma unroll
+      for (int k = 0; k < V; ++k) st.v[k] = 0.f;
+      if (t.in && q0 < a.T) st = ldv<float, V>(a.states + (int64_t)(q0 / kPiece) * a.R * a.H + t.ch);
+#pragma unroll
+      for (int k = 0; k < V; ++k) hp[k] = st.v[k];
+    }
+    float u[kPiece][V], e[kPiece][V], dgf[kPiece][V], vv[kPiece][V];  // e: dh; dgf: (h_{t-1} - c) u v
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) {
+      const bool on = q0 + i >= t.lo && q0 + i < t.hi;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        float uu, v1;
+        gate_uv(ld1(ra[i].v[k]), uu, v1);
+        u[i][k] = on ? uu : 1.f;
+        e[i][k] = on && d ? ld1(rd[i].v[k]) : 0.f;
+        if constexpr (!SUM) {
+          const float cc = ld1(rb[i].v[k]);
+          dgf[i][k] = on ? (hp[k] - cc) * (uu * v1) : 0.f;
+          vv[i][k] = on ? v1 : 0.f;
+          hp[k] = on ? fmaf(uu, hp[k], v1 * cc) : hp[k];
+        }
+      }
+    }
+    float gam[V];
+    if constexpr (NW > 1) {
+      float P[V], Q[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        P[k] = 1.f;
+        Q[k] = 0.f;
+      }
+#pragma unroll
+      for (int i = kPiece - 1; i >= 0; --i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          Q[k] = u[i][k] * (e[i][k] + Q[k]);
+          P[k] *= u[i][k];
+        }
+      // an active step's dh joins g in front of its u; a step that does not act has u = 1 and dh = 0
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        lds[buf][w][lane][k] = P[k];
+        lds[buf][w][lane][V + k] = Q[k];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = NW - 1; j >= 0; --j)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          if (j == w) gam[k] = carry[k];
+          carry[k] = fmaf(lds[buf][j][lane][k], carry[k], lds[buf][j][lane][V + k]);
+          if constexpr (SUM) span[k] *= lds[buf][j][lane][k];
+        }
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) gam[k] = carry[k];
+    }
+    if constexpr (!SUM) {
+      if (t.in && q0 < a.T) {
+#pragma unroll
+        for (int i = kPiece - 1; i >= 0; --i) {
+          const int p = q0 + i;
+          Pack<T, V> pg, pc;
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const float gg = e[i][k] + gam[k];
+            // a step that does not act passes gamma on as it is; its own gradients are zero whatever gamma is
+            const bool on = p >= t.lo && p < t.hi;
+            pg.v[k] = st1<T>(on ? gg * dgf[i][k] : 0.f);
+            pc.v[k] = st1<T>(on ? gg * vv[i][k] : 0.f);
+            gam[k] = u[i][k] * gg;
+          }
+          if (p < a.T) {
+            stv<T, V>(og + sg * p * a.ogt, pg);
+            stv<T, V>(oc + sg * p * a.oct, pc);
+          }
+        }
+      }
+      if constexpr (NW == 1) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) carry[k] = gam[k];
+      }
+    }
+  }
+  if (!t.in || w) return;
+  if constexpr (SUM) {
+    const int64_t C = a.R * a.H;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      a.sums[(int64_t)s * C + t.ch + k] = span[k];
+      a.sums[(int64_t)(a.S + s) * C + t.ch + k] = carry[k];
+    }
+  } else if (begin == 0 && a.dh0) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) a.dh0[t.ch + k] = carry[k];
+  }
+}
+
+// ---- one token ---------------------------------------------------------------------------------
+template <typename T, int V>
+__global__ __launch_bounds__(256) void k_recur_step(const T* __restrict__ gate, int64_t gr, const T* __restrict__ cand,
+                                                    int64_t cr, float* __restrict__ state, int64_t sr, T* __restrict__ h,
+                                                    int64_t hr, int64_t R, int H, int upr) {
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= R * upr) return;
+  const int64_t r = u / upr;
+  const int c = (int)(u - r * upr) * V;
+  const Pack<T, V> a = ldv<T, V>(gate + r * gr + c), b = ldv<T, V>(cand + r * cr + c);
+  Pack<float, V> s = ldv<float, V>(state + r * sr + c);
+  Pack<T, V> o;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    float uu, vv;
+    gate_uv(ld1(a.v[k]), uu, vv);
+    s.v[k] = fmaf(uu, s.v[k], vv * ld1(b.v[k]));
+    o.v[k] = st1<T>(s.v[k]);
+  }
+  stv<float, V>(state + r * sr + c, s);
+  stv<T, V>(h + r * hr + c, o);
+}
+
+// How the work is cut.  `waves`: waves of 64 lanes that the channels alone give.
+struct Cut {
+  int V, NW, S, L;
+};
+Cut cut_of(int64_t R, int T, int H, int dtype) {
+  Cut c{};
+  const int wide = dtype == DSSM_F32 ? 1 : 2;
+  c.V = H % wide ? 1 : wide;
+  const int64_t waves = (R * (H / c.V) + 63) / 64;
+  const int pieces = (T + kPiece - 1) / kPiece;
+  c.NW = 1;
+  c.S = 1;
+  if (waves < 1024 && pieces > 1) {
+    c.NW = pieces >= 5 ? 8 : 4;
+    const int64_t want = 2048 / (waves * c.NW);
+    if (want >= 2) c.S = (int)std::min<int64_t>(want, (pieces + 2 * c.NW - 1) / (2 * c.NW));
+  }
+  const int round = c.NW * kPiece, per = (T + c.S - 1) / c.S;
+  c.L = (per + round - 1) / round * round;
+  c.S = (T + c.L - 1) / c.L;
+  return c;
+}
+
+bool recur_dims_ok(int64_t R, int T, int H) {
+  return R > 0 && T > 0 && H > 0 && T <= (1 << 28) && H <= (1 << 20) && R <= ((int64_t)1 << 31) &&
+         (R * H + 63) / 64 <= 0x7fffffff;
+}
+
+template <typename T, int V, bool FWD>
+void launch(const RecurArgs& a, const Cut& c, hipStream_t s) {
+  const dim3 grid((unsigned)((a.R * a.upr + 63) / 64), (unsigned)c.S);
+  auto go = [&](auto nw) {
+    constexpr int NW = decltype(nw)::value;
+    if constexpr (FWD) {
+      if constexpr (NW > 1)
+        if (c.S > 1) hipLaunchKernelGGL((k_recur_fwd<T, V, NW, true>), grid, dim3(NW * 64), 0, s, a);
+      hipLaunchKernelGGL((k_recur_fwd<T, V, NW, false>), grid, dim3(NW * 64), 0, s, a);
+    } else {
+      if constexpr (NW > 1)
+        if (c.S > 1) hipLaunchKernelGGL((k_recur_bwd<T, V, NW, true>), grid, dim3(NW * 64), 0, s, a);
+      hipLaunchKernelGGL((k_recur_bwd<T, V, NW, false>), grid, dim3(NW * 64), 0, s, a);
+    }
+  };
+  if (c.NW == 1) go(std::integral_constant<int, 1>{});
+  else if (c.NW == 4) go(std::integral_constant<int, 4>{});
+  else go(std::integral_constant<int, 8>{});
+}
+template <bool FWD>
+int run(RecurArgs& a, int dtype, void* stream) {
+  const Cut c = cut_of(a.R, a.T, a.H, dtype);
+  a.upr = a.H / c.V;
+  a.S = c.S;
+  a.L = c.L;
+  by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    if constexpr (sizeof(T) == 4) {
+      launch<T, 1, FWD>(a, c, (hipStream_t)stream);
+    } else {
+      if (c.V == 2) launch<T, 2, FWD>(a, c, (hipStream_t)stream);
+      else launch<T, 1, FWD>(a, c, (hipStream_t)stream);
+    }
+  });
+  return seq_status(hipGetLastError());
+}
+
+}  // namespace
+}  // namespace seq
+}  // namespace dssm
+
+using namespace dssm::seq;
+
+extern "C" size_t dssm_linear_recurrence_ws_bytes(int64_t R, int T, int H, int dtype) {
+  if (!recur_dims_ok(R, T, H) || !seq_dtype(dtype)) return 0;
+  const Cut c = cut_of(R, T, H, dtype);
+  return c.S > 1 ? (size_t)2 * c.S * R * H * sizeof(float) : 0;
+}
+
+extern "C" int dssm_linear_recurrence(const void* gate, int64_t gr, int64_t gt, const void* cand, int64_t cr, int64_t ct,
+                                      int dtype, const int32_t* lens, const float* h0, int64_t R, int T, int H,
+                                      int reverse, void* h, int64_t hr, int64_t ht, float* last, float* states, void* ws,
+                                      size_t ws_bytes, void* stream) {
+  if (!gate || !cand || !h || !last || !seq_dtype(dtype) || !recur_dims_ok(R, T, H))
+    return dssm::report_error(DSSM_E_INVALID, "linear_recurrence: bad argument");
+  const size_t need = dssm_linear_recurrence_ws_bytes(R, T, H, dtype);
+  if (need && (!ws || ws_bytes < need))
+    return dssm::report_error(DSSM_E_INVALID, "linear_recurrence: workspace too small (dssm_linear_recurrence_ws_bytes)");
+  RecurArgs a{};
+  a.gate = gate;
+  a.cand = cand;
+  a.gr = gr;
+  a.gt = gt;
+  a.cr = cr;
+  a.ct = ct;
+  a.lens = lens;
+  a.h0 = h0;
+  a.h = h;
+  a.hr = hr;
+  a.ht = ht;
+  a.last = last;
+  a.states = states;
+  a.sums = (float*)ws;
+  a.R = R;
+  a.T = T;
+  a.H = H;
+  a.reverse = reverse != 0;
+  return run<true>(a, dtype, stream);
+}
+
+extern "C" int dssm_linear_recurrence_bwd(const void* gate, int64_t gr, int64_t gt, const void* cand, int64_t cr,
+                                          int64_t ct, int dtype, const int32_t* lens, const float* states, const void* dh,
+                                          int64_t dr, int64_t dt, const float* dlast, int64_t R, int T, int H, int reverse,
+                                          void* dgate, int64_t ogr, int64_t ogt, void* dcand, int64_t ocr, int64_t oct,
+                                          float* dh0, void* ws, size_t ws_bytes, void* stream) {
+  if (!gate || !cand || !states || !dgate || !dcand || !seq_dtype(dtype) || !recur_dims_ok(R, T, H))
+    return dssm::report_error(DSSM_E_INVALID, "linear_recurrence_bwd: bad argument");
+  const size_t need = dssm_linear_recurrence_ws_bytes(R, T, H, dtype);
+  if (need && (!ws || ws_bytes < need))
+    return dssm::report_error(DSSM_E_INVALID, "linear_recurrence_bwd: workspace too small (dssm_linear_recurrence_ws_bytes)");
+  RecurArgs a{};
+  a.gate = gate;
+  a.cand = cand;
+  a.dh = dh;
+  a.gr = gr;
+  a.gt = gt;
+  a.cr = cr;
+  a.ct = ct;
+  a.dr = dr;
+  a.dt = dt;
+  a.lens = lens;
+  a.dlast = dlast;
+  a.states = const_cast<float*>(states);
+  a.dgate = dgate;
+  a.dcand = dcand;
+  a.ogr = ogr;
+  a.ogt = ogt;
+  a.ocr = ocr;
+  a.oct = oct;
+  a.dh0 = dh0;
+  a.sums = (float*)ws;
+  a.R = R;
+  a.T = T;
+  a.H = H;
+  a.reverse = reverse != 0;
+  return run<false>(a, dtype, stream);
+}
+
+extern "C" int dssm_linear_recurrence_step(const void* gate, int64_t gr, const void* cand, int64_t cr, int dtype,
+                                           float* state, int64_t sr, void* h, int64_t hr, int64_t R, int H, void* stream) {
+  if (!gate || !cand || !state || !h || !seq_dtype(dtype) || !recur_dims_ok(R, 1, H))
+    return dssm::report_error(DSSM_E_INVALID, "linear_recurrence_step: bad argument");
+  by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    auto go = [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      const int64_t units = R * (H / V);
+      hipLaunchKernelGGL((k_recur_step<T, V>), dim3((unsigned)((units + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+                         (const T*)gate, gr, (const T*)cand, cr, state, sr, (T*)h, hr, R, H, H / V);
+    };
+    if (H % 4 == 0) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 1>{});
+  });
+  return seq_status(hipGetLastError());
+}

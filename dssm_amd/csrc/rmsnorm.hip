@@ -1,0 +1,419 @@
+// Root-mean-square norm with the residual's addition, its output in the input's type or in the 8-bit block
+// form, its gradient; and the 8-bit block form of plain rows and back.
+//
+//   s = round(x + residual),  rstd = 1 / sqrt(mean s^2 + eps),  y = s rstd w
+//   n = s rstd:  dx = rstd (w dy - n mean(w dy n)) + ds,   dw = sum over rows of dy n
+//
+// s is rounded to its storage type before the norm, so that the backward, which reads the stored s, is
+// the gradient of exactly this forward.  All sums are fp32.
+//
+// Every kernel here is one pass over its rows, bound by memory.  A row stays in registers: NT threads (a
+// quarter wave to a workgroup of 16 waves) hold 8 neighbouring columns each, K times over; 16 lanes hold a
+// block of 128 columns, so a block's scale is four DPP steps away.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "seq.h"
+
+namespace dssm {
+namespace seq {
+namespace {
+
+constexpr int kMaxCols = 16384;  // 1024 threads x 8 columns x 2
+
+// the sum of v over the NT threads that share a row (every thread gets it); s: one float a wave
+template <int NT>
+__device__ __forceinline__ float row_sum(float v, float* s) {
+  v = wave_allsum_step<0>(v);
+  v = wave_allsum_step<1>(v);
+  v = wave_allsum_step<2>(v);
+  v = wave_allsum_step<3>(v);
+  if constexpr (NT >= 64) {
+    v = wave_allsum_step<4>(v);
+    v = wave_allsum_step<5>(v);
+  }
+  if constexpr (NT > 64) {
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) s[w] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) v += s[i];
+    __syncthreads();
+  }
+  return v;
+}
+
+struct NormArgs {
+  const void *x, *res, *dy, *ds, *s_in;
+  int64_t ldx, ldres, lddy, ldds, lds;
+  const float *w, *rstd_in;
+  void *y, *s, *dx;
+  int64_t ldy, lddx;
+  float* rstd;
+  unsigned char *q, *scale;  // 8-bit form: q [rows x Kp], scale [rows x Kp / 128]
+  float* part;               // backward: [blocks x cols]
+  int64_t rows;
+  int cols, kp;
+  float eps;
+};
+
+// MODE 0: y in T; 1: y in the 8-bit form; 2: x itself in the 8-bit form (no norm)
+template <typename T, int NT, int K, int MODE>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
+  constexpr int kRows = NT < 256 ? 256 / NT : 1;
+  __shared__ float red[16];
+  const int l = threadIdx.x % NT;
+  const int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / NT;
+  const bool in = r < a.rows;
+  float v[K][8];
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * NT + l) * 8, nv = a.cols - c;
+    if (in && nv > 0) {
+      ld_row<T, 8>((const T*)a.x + r * a.ldx + c, nv, v[k]);
+      if (MODE != 2 && a.res) {
+        float b[8];
+        ld_row<T, 8>((const T*)a.res + r * a.ldres + c, nv, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[k][i] = ld1(st1<T>(v[k][i] + b[i]));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
+    }
+    if constexpr (MODE != 2) {
+      if (in && nv > 0 && a.s) st_row<T, 8>((T*)a.s + r * a.lds + c, nv, v[k]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(v[k][i], v[k][i], sum);
+    }
+  }
+  if constexpr (MODE != 2) {
+    const float rstd = 1.0f / sqrtf(row_sum<NT>(sum, red) / (float)a.cols + a.eps);
+    if (in && l == 0 && a.rstd) a.rstd[r] = rstd;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * NT + l) * 8, nv = a.cols - c;
+      if (nv <= 0) continue;
+      float w[8];
+      ld_row<float, 8>(a.w + c, nv, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[k][i] = i < nv ? v[k][i] * rstd * w[i] : 0.f;  // the form's padding is zero
+      if (MODE == 0 && in) st_row<T, 8>((T*)a.y + r * a.ldy + c, nv, v[k]);
+    }
+  }
+  if constexpr (MODE != 0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * NT + l) * 8;
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(v[k][i]));
+      const unsigned e = blk_exp(max16(m));
+      if (in && c < a.kp) {
+        *reinterpret_cast<uint2*>(a.q + r * a.kp + c) = to_e4m3x8(v[k], exp_inv(e));
+        if ((l & 15) == 0) a.scale[r * (a.kp / kBlk) + c / kBlk] = (unsigned char)e;
+      }
+    }
+  }
+}
+
+// Backward.  A workgroup walks rows blockIdx.x * kRows + i * gridDim.x * kRows and keeps its share of dw in
+// registers; its rows' slots meet in LDS at the end and the workgroup leaves one partial row.
+template <typename T, int NT, int K>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_bwd(NormArgs a) {
+  constexpr int kRows = NT < 256 ? 256 / NT : 1;
+  __shared__ float red[16];
+  __shared__ float slot[kRows > 1 ? kRows : 1][kRows > 1 ? NT * 8 + 4 : 1];
+  const int l = threadIdx.x % NT, g = threadIdx.x / NT;
+  float w[K][8], dw[K][8];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * NT + l) * 8, nv = a.cols - c;
+    if (nv > 0) {
+      ld_row<float, 8>(a.w + c, nv, w[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[k][i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[k][i] = 0.f;
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < a.rows; r0 += (int64_t)gridDim.x * kRows) {
+    const int64_t r = r0 + g;
+    const bool in = r < a.rows;
+    const float rstd = in ? a.rstd_in[r] : 0.f;
+    float n[K][8], d[K][8], sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * NT + l) * 8, nv = a.cols - c;
+      if (in && nv > 0) {
+        ld_row<T, 8>((const T*)a.s_in + r * a.lds + c, nv, n[k]);
+        ld_row<T, 8>((const T*)a.dy + r * a.lddy + c, nv, d[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n[k][i] = d[k][i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        n[k][i] *= rstd;
+        dw[k][i] = fmaf(d[k][i], n[k][i], dw[k][i]);
+        d[k][i] *= w[k][i];
+        sum = fmaf(d[k][i], n[k][i], sum);
+      }
+    }
+    const float mean = row_sum<NT>(sum, red) / (float)a.cols;
+    if (!in) continue;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * NT + l) * 8, nv = a.cols - c;
+      if (nv <= 0) continue;
+      float o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = rstd * (d[k][i] - n[k][i] * mean);
+      if (a.ds) {
+        float b[8];
+        ld_row<T, 8>((const T*)a.ds + r * a.ldds + c, nv, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] += b[i];
+      }
+      st_row<T, 8>((T*)a.dx + r * a.lddx + c, nv, o);
+    }
+  }
+  float* out = a.part + (int64_t)blockIdx.x * a.cols;
+  if constexpr (kRows > 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) slot[g][l * 8 + i] = dw[k][i];
+      __syncthreads();
+      for (int j = threadIdx.x; j < NT * 8; j += 256) {
+        float t = 0.f;
+#pragma unroll
+        for (int q = 0; q < kRows; ++q) t += slot[q][j];
+        const int c = k * NT * 8 + j;
+        if (c < a.cols) out[c] = t;
+      }
+      __syncthreads();
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * NT + l) * 8, nv = a.cols - c;
+      if (nv > 0) st_row<float, 8>(out + c, nv, dw[k]);
+    }
+  }
+}
+
+// dw [cols] = the partial rows' sum, in order: 16 columns a workgroup, 64 stretches of the rows each
+__global__ __launch_bounds__(1024) void k_norm_dw(const float* __restrict__ part, int blocks, int cols,
+                                                  float* __restrict__ dw) {
+  __shared__ float red[64][17];
+  const int j = threadIdx.x & 15, t = threadIdx.x >> 4, c = blockIdx.x * 16 + j;
+  const int per = (blocks + 63) / 64, b0 = min(t * per, blocks), b1 = min(b0 + per, blocks);
+  float v = 0.f;
+  if (c < cols)
+    for (int b = b0; b < b1; ++b) v += part[(int64_t)b * cols + c];
+  red[t][j] = v;
+  __syncthreads();
+  if (t == 0 && c < cols) {
+    float sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < 64; ++q) sum += red[q][j];
+    dw[c] = sum;
+  }
+}
+
+// the 8-bit form's values: 8 columns a thread
+template <typename O>
+__global__ __launch_bounds__(256) void k_dequant(const unsigned char* __restrict__ q, const unsigned char* __restrict__ scale,
+                                                 int64_t rows, int cols, int kp, O* __restrict__ out, int64_t ldo) {
+  const int per = (cols + 7) / 8;
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= rows * per) return;
+  const int64_t r = u / per;
+  const int c = (int)(u - r * per) * 8;
+  const uint2 b = *reinterpret_cast<const uint2*>(q + r * kp + c);
+  const unsigned e = scale[r * (kp / kBlk) + c / kBlk];
+  const float s = e == 255u ? __builtin_nanf("") : exp_val(e);
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int v = (int)(i ? b.y : b.x);
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(v, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
+    x[4 * i] = lo[0] * s;
+    x[4 * i + 1] = lo[1] * s;
+    x[4 * i + 2] = hi[0] * s;
+    x[4 * i + 3] = hi[1] * s;
+  }
+  st_row<O, 8>(out + r * ldo + c, cols - c, x);
+}
+
+// Threads a row: the fewest that hold it, but a whole workgroup for wide rows, whose wave would keep too
+// few loads in flight.
+template <typename F>
+void by_cols(int cols, F&& f) {
+  using std::integral_constant;
+  if (cols <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  else if (cols <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+  else if (cols <= 8192) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+  else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+}
+
+bool norm_dims_ok(int64_t rows, int cols) {
+  return rows >= 0 && rows <= 0x7fffffff && cols > 0 && cols <= kMaxCols;
+}
+int kp_of(int cols) { return (cols + kBlk - 1) / kBlk * kBlk; }
+
+template <int MODE>
+void run_norm(const NormArgs& a, int dtype, hipStream_t s) {
+  by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    by_cols(a.cols, [&](auto nt, auto kk) {
+      constexpr int NT = decltype(nt)::value, K = decltype(kk)::value, rows = NT < 256 ? 256 / NT : 1;
+      hipLaunchKernelGGL((k_norm<T, NT, K, MODE>), dim3((unsigned)((a.rows + rows - 1) / rows)),
+                         dim3(NT < 256 ? 256 : NT), 0, s, a);
+    });
+  });
+}
+constexpr int kBwdBlocks = 1024;  // partial rows of dw at most
+int bwd_blocks(int64_t rows, int cols) {
+  const int per = cols <= 128 ? 16 : cols <= 1024 ? 4 : 1;  // rows a workgroup takes at once
+  return (int)std::max<int64_t>(1, std::min<int64_t>(kBwdBlocks, (rows + per - 1) / per));
+}
+
+}  // namespace
+}  // namespace seq
+}  // namespace dssm
+
+using namespace dssm::seq;
+
+extern "C" int dssm_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldres, const float* weight,
+                             int64_t rows, int cols, int dtype, float eps, void* y, int64_t ldy, void* s, int64_t lds,
+                             float* rstd, void* stream) {
+  if (!seq_dtype(dtype) || !norm_dims_ok(rows, cols) || !weight || ldx < cols || ldy < cols || (residual && ldres < cols) ||
+      (s && lds < cols) || (rows > 0 && (!x || !y)))
+    return dssm::report_error(DSSM_E_INVALID, "rms_norm: bad argument (1 to 16384 columns)");
+  if (rows == 0) return DSSM_OK;
+  NormArgs a{};
+  a.x = x;
+  a.ldx = ldx;
+  a.res = residual;
+  a.ldres = ldres;
+  a.w = weight;
+  a.rows = rows;
+  a.cols = cols;
+  a.eps = eps;
+  a.y = y;
+  a.ldy = ldy;
+  a.s = s;
+  a.lds = lds;
+  a.rstd = rstd;
+  run_norm<0>(a, dtype, (hipStream_t)stream);
+  return seq_status(hipGetLastError());
+}
+
+extern "C" int dssm_rms_norm_blocks8(const void* x, int64_t ldx, const void* residual, int64_t ldres, const float* weight,
+                                     int64_t rows, int cols, int dtype, float eps, void* q, void* scale, void* s,
+                                     int64_t lds, float* rstd, void* stream) {
+  if (!seq_dtype(dtype) || !norm_dims_ok(rows, cols) || !weight || ldx < cols || (residual && ldres < cols) ||
+      (s && lds < cols) || (rows > 0 && (!x || !q || !scale)) || (uintptr_t)q % 16)
+    return dssm::report_error(DSSM_E_INVALID, "rms_norm_blocks8: bad argument (1 to 16384 columns, 16-byte aligned values)");
+  if (rows == 0) return DSSM_OK;
+  NormArgs a{};
+  a.x = x;
+  a.ldx = ldx;
+  a.res = residual;
+  a.ldres = ldres;
+  a.w = weight;
+  a.rows = rows;
+  a.cols = cols;
+  a.kp = kp_of(cols);
+  a.eps = eps;
+  a.q = (unsigned char*)q;
+  a.scale = (unsigned char*)scale;
+  a.s = s;
+  a.lds = lds;
+  a.rstd = rstd;
+  run_norm<1>(a, dtype, (hipStream_t)stream);
+  return seq_status(hipGetLastError());
+}
+
+extern "C" size_t dssm_rms_norm_bwd_ws_bytes(int64_t rows, int cols) {
+  return norm_dims_ok(rows, cols) ? (size_t)bwd_blocks(rows, cols) * cols * sizeof(float) + 16 : 0;
+}
+
+extern "C" int dssm_rms_norm_bwd(const void* dy, int64_t lddy, const void* s, int64_t lds, const float* weight,
+                                 const float* rstd, const void* ds, int64_t ldds, int64_t rows, int cols, int dtype, void* dx,
+                                 int64_t lddx, float* dweight, void* ws, size_t ws_bytes, void* stream) {
+  if (!seq_dtype(dtype) || !norm_dims_ok(rows, cols) || !weight || !dweight || lddy < cols || lds < cols || lddx < cols ||
+      (ds && ldds < cols) || (rows > 0 && (!dy || !s || !rstd || !dx)))
+    return dssm::report_error(DSSM_E_INVALID, "rms_norm_bwd: bad argument (1 to 16384 columns)");
+  if (!ws || ws_bytes < dssm_rms_norm_bwd_ws_bytes(rows, cols))
+    return dssm::report_error(DSSM_E_INVALID, "rms_norm_bwd: workspace too small (dssm_rms_norm_bwd_ws_bytes)");
+  hipStream_t st = (hipStream_t)stream;
+  NormArgs a{};
+  a.dy = dy;
+  a.lddy = lddy;
+  a.s_in = s;
+  a.lds = lds;
+  a.w = weight;
+  a.rstd_in = rstd;
+  a.ds = ds;
+  a.ldds = ldds;
+  a.rows = rows;
+  a.cols = cols;
+  a.dx = dx;
+  a.lddx = lddx;
+  a.part = (float*)ws;
+  const int blocks = bwd_blocks(rows, cols);
+  by_dtype(dtype, [&](auto tag) {
+    using T = decltype(tag);
+    by_cols(cols, [&](auto nt, auto kk) {
+      constexpr int NT = decltype(nt)::value, K = decltype(kk)::value;
+      hipLaunchKernelGGL((k_norm_bwd<T, NT, K>), dim3(blocks), dim3(NT < 256 ? 256 : NT), 0, st, a);
+    });
+  });
+  hipLaunchKernelGGL(k_norm_dw, dim3((cols + 15) / 16), dim3(1024), 0, st, (const float*)ws, blocks, cols, dweight);
+  return seq_status(hipGetLastError());
+}
+
+extern "C" int dssm_quantize_blocks8(const void* x, int64_t ldx, int64_t rows, int cols, int dtype, void* q, void* scale,
+                                     void* stream) {
+  if (!seq_dtype(dtype) || !norm_dims_ok(rows, cols) || ldx < cols || (rows > 0 && (!x || !q || !scale)) ||
+      (uintptr_t)q % 16)
+    return dssm::report_error(DSSM_E_INVALID, "quantize_blocks8: bad argument (1 to 16384 columns, 16-byte aligned values)");
+  if (rows == 0) return DSSM_OK;
+  NormArgs a{};
+  a.x = x;
+  a.ldx = ldx;
+  a.rows = rows;
+  a.cols = cols;
+  a.kp = kp_of(cols);
+  a.q = (unsigned char*)q;
+  a.scale = (unsigned char*)scale;
+  run_norm<2>(a, dtype, (hipStream_t)stream);
+  return seq_status(hipGetLastError());
+}
+
+extern "C" int dssm_dequantize_blocks8(const void* q, const void* scale, int64_t rows, int cols, void* out, int64_t ldo,
+                                       int out_dtype, void* stream) {
+  if (!seq_dtype(out_dtype) || !norm_dims_ok(rows, cols) || ldo < cols || (rows > 0 && (!out || !q || !scale)) ||
+      (uintptr_t)q % 16)
+    return dssm::report_error(DSSM_E_INVALID, "dequantize_blocks8: bad argument (1 to 16384 columns, 16-byte aligned values)");
+  if (rows == 0) return DSSM_OK;
+  const int64_t units = rows * ((cols + 7) / 8);
+  if ((units + 255) / 256 > 0x7fffffff) return dssm::report_error(DSSM_E_UNSUPPORTED, "dequantize_blocks8: too many values");
+  by_dtype(out_dtype, [&](auto tag) {
+    using O = decltype(tag);
+    hipLaunchKernelGGL(k_dequant<O>, dim3((unsigned)((units + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+                       (const unsigned char*)q, (const unsigned char*)scale, rows, cols, kp_of(cols), (O*)out, ldo);
+  });
+  return seq_status(hipGetLastError());
+}

@@ -33,7 +33,7 @@ extern "C" {
 #define DSSM_MAX_LAYERS 8
 
 enum { DSSM_OK = 0, DSSM_E_INVALID = -1, DSSM_E_HIP = -2, DSSM_E_RCCL = -3, DSSM_E_UNSUPPORTED = -4 };
-enum { DSSM_F32 = 0, DSSM_BF16 = 1, DSSM_I32 = 2 /* collectives only */ };
+enum { DSSM_F32 = 0, DSSM_BF16 = 1, DSSM_I32 = 2 /* collectives only */, DSSM_F16 = 3 /* sequence operators only */ };
 
 /* Model/step configuration (semantic_matching/dssm/config.py:19-28 + new_dssm.py constants). */
 typedef struct dssm_config {
@@ -689,6 +689,80 @@ int dssm_rnn_adam(float* p, const float* g, float* m, float* v, int64_t n_sparse
  * recurrences' embedding copy, kept current by the optimizer. */
 int dssm_rnn_adam_ex(float* p, const float* g, float* m, float* v, int64_t n_sparse, int64_t n,
                      float* state, float lr, float beta1, float beta2, float eps, uint16_t* shadow, void* stream);
+
+/* ---- sequence-tower operators (dssm_amd/seqops.py; csrc/embed.hip, linrec.hip, rmsnorm.hip, gemm8.hip) ----
+ * The pieces of a gated recurrent tower over token ids beside the GRU tower (dssm_rnn.py:100-217): its
+ * lookup, a recurrence whose gates do not look at the state (so that time can be cut), the norm between
+ * layers, and the 8-bit product.  Storage types dtype / out_dtype: DSSM_F32, DSSM_BF16, DSSM_F16; sums,
+ * statistics and states are fp32.  Leading dimensions and strides are in elements, rows may start at any
+ * element.  Sizes of zero rows do nothing.  Outputs must not overlap inputs unless a call says so. */
+
+/* tf.nn.embedding_lookup(table, ids) * scale (dssm_rnn.py:113-118): out [n x E] from table [V x E] (row
+ * stride ldt).  ids: int32, or int64 with ids64; an id outside [0, V) gives a row of zeros. */
+int dssm_embedding_lookup(const void* table, int dtype, int64_t ldt, int64_t V, int E, const void* ids, int ids64,
+                          int64_t n, float scale, void* out, int out_dtype, void* stream);
+/* Its gradient: dtable [V x E] fp32 (16-byte aligned, every row written) = scale * the rows of dy [n x E]
+ * summed by token, in the order of their positions (the result does not depend on timing); ids outside
+ * [0, V) are left out.  n < 2^31 - 4096, V < 2^30, E <= 2^20.  ws: dssm_embedding_grad_ws_bytes() bytes,
+ * 16-byte aligned, of any content (0: a size is out of range). */
+size_t dssm_embedding_grad_ws_bytes(int64_t n, int64_t V, int E);
+int dssm_embedding_grad(const void* dy, int dtype, int64_t lddy, const void* ids, int ids64, int64_t n, int64_t V, int E,
+                        float scale, float* dtable, void* ws, size_t ws_bytes, void* stream);
+
+/* Gated linear recurrence over [R x T x H]: u = sigmoid(gate), h_t = u_t h_{t-1} + (1 - u_t) cand_t (the
+ * GRUCell's convention without its state-dependent gates).  Row and time strides of gate, cand and h are
+ * free (both halves of one projection, time-major storage).  lens [R] (NULL: T; clamped to [0, T]): steps
+ * at or past it are not read, emit zero and carry the state.  reverse: from the row's last step to its
+ * first.  h0 [R x H] fp32 or NULL (zeros); last [R x H] fp32: the state after the walk.  states (NULL for
+ * inference): ceil(T / DSSM_RECUR_PIECE) x R x H floats, the state in front of every DSSM_RECUR_PIECE steps of
+ * the walk, read by the backward.  ws: dssm_linear_recurrence_ws_bytes() bytes of any content (0: none
+ * is needed, ws may be NULL); forward and backward need the same. */
+#define DSSM_RECUR_PIECE 16
+size_t dssm_linear_recurrence_ws_bytes(int64_t R, int T, int H, int dtype);
+int dssm_linear_recurrence(const void* gate, int64_t gate_row, int64_t gate_time, const void* cand, int64_t cand_row,
+                           int64_t cand_time, int dtype, const int32_t* lens, const float* h0, int64_t R, int T, int H,
+                           int reverse, void* h, int64_t h_row, int64_t h_time, float* last, float* states, void* ws,
+                           size_t ws_bytes, void* stream);
+/* Gradient of the above for dh [R x T x H] (NULL: zero; not read past a row's length) and dlast [R x H]
+ * (NULL: zero): dgate, dcand (zero past a row's length) and dh0 [R x H] (NULL: not wanted).  gate, cand,
+ * lens and reverse as the forward had them. */
+int dssm_linear_recurrence_bwd(const void* gate, int64_t gate_row, int64_t gate_time, const void* cand, int64_t cand_row,
+                               int64_t cand_time, int dtype, const int32_t* lens, const float* states, const void* dh,
+                               int64_t dh_row, int64_t dh_time, const float* dlast, int64_t R, int T, int H, int reverse,
+                               void* dgate, int64_t dgate_row, int64_t dgate_time, void* dcand, int64_t dcand_row,
+                               int64_t dcand_time, float* dh0, void* ws, size_t ws_bytes, void* stream);
+/* One step for R rows: state [R x H] fp32 in place, h [R x H] = the new state in the inputs' type. */
+int dssm_linear_recurrence_step(const void* gate, int64_t ldgate, const void* cand, int64_t ldcand, int dtype,
+                                float* state, int64_t ldstate, void* h, int64_t ldh, int64_t R, int H, void* stream);
+
+/* Root-mean-square norm of s = x + residual (rounded to dtype; residual NULL: s = x): rstd = 1 /
+ * sqrt(mean s^2 + eps), y = s * rstd * weight.  s (NULL: not wanted; may be x or residual itself) and rstd
+ * [rows] (NULL: not wanted) are what the backward reads.  weight [cols] fp32, 1 to 16384 columns. */
+int dssm_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldres, const float* weight, int64_t rows,
+                  int cols, int dtype, float eps, void* y, int64_t ldy, void* s, int64_t lds, float* rstd, void* stream);
+/* Gradient: dx (= d residual) = the norm's gradient of dy at s, plus ds (NULL: none; the gradient that
+ * reaches s past the norm; dx may be ds or dy itself); dweight [cols] fp32, summed in a fixed order. */
+size_t dssm_rms_norm_bwd_ws_bytes(int64_t rows, int cols);
+int dssm_rms_norm_bwd(const void* dy, int64_t lddy, const void* s, int64_t lds, const float* weight, const float* rstd,
+                      const void* ds, int64_t ldds, int64_t rows, int cols, int dtype, void* dx, int64_t lddx,
+                      float* dweight, void* ws, size_t ws_bytes, void* stream);
+
+/* The 8-bit block form of [rows x K]: q [rows x Kp] e4m3 (Kp = K rounded up to 128, padding zero, 16-byte
+ * aligned) and scale [rows x Kp / 128] E8M0 bytes: a row's block of 128 columns stands for q * 2^(byte -
+ * 127), the smallest power of two that brings the block's largest finite magnitude into +-448 (2^0 for a
+ * block of zeros).  Values round to nearest even; NaN and infinities become NaN. */
+int dssm_quantize_blocks8(const void* x, int64_t ldx, int64_t rows, int cols, int dtype, void* q, void* scale, void* stream);
+int dssm_dequantize_blocks8(const void* q, const void* scale, int64_t rows, int cols, void* out, int64_t ldo, int out_dtype,
+                            void* stream);
+/* dssm_rms_norm with y in the 8-bit block form. */
+int dssm_rms_norm_blocks8(const void* x, int64_t ldx, const void* residual, int64_t ldres, const float* weight, int64_t rows,
+                          int cols, int dtype, float eps, void* q, void* scale, void* s, int64_t lds, float* rstd,
+                          void* stream);
+/* add_layer (README.md:66-76) of two operands in the 8-bit block form: out [M x N] = a [M x K] * w [N x K]^T
+ * (+ bias [N] fp32 or NULL), out_dtype DSSM_BF16 or DSSM_F16.  Products join an fp32 sum in eights, which the
+ * matrix unit adds on a grid of 2^-13 of their largest. */
+int dssm_blocks8_matmul(const void* a, const void* ascale, const void* w, const void* wscale, int64_t M, int64_t N, int64_t K,
+                        const float* bias, void* out, int64_t ldo, int out_dtype, void* stream);
 
 #ifdef __cplusplus
 }
