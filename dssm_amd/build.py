@@ -21,6 +21,8 @@ HEADERS = ["common.h", "launch.h", "gather.h", "bnfuse.h", "flat.h", "tn.h", "cs
 ARCH = os.environ.get("DSSM_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function"]
+# no packed fp32 instructions: some of their forms have given wrong results on this part now and then
+CFLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 CFLAGS += os.environ.get("DSSM_EXTRA_CFLAGS", "").split()  # diagnostics builds (e.g. -DDSSM_WG_TL)
 
 
