@@ -230,7 +230,7 @@ _SIGS = {
     "dssm_plan_peer_selftest": (C.c_int, [_P, _P, _P]),
     # sequence-tower operators (dssm_amd/seqops.py)
     "dssm_embedding_lookup": (C.c_int, [_P, C.c_int, _L, _L, C.c_int, _P, C.c_int, _L, C.c_float, _P, C.c_int, _P]),
-    "dssm_embedding_grad_ws_bytes": (C.c_size_t, [_L, _L, C.c_int]),
+    "dssm_embedding_grad_ws_bytes": (C.c_size_t, [_L, _L, C.c_int, C.c_int]),
     "dssm_embedding_grad": (C.c_int, [_P, C.c_int, _L, _P, C.c_int, _L, _L, C.c_int, C.c_float, _P, _P, C.c_size_t, _P]),
     "dssm_linear_recurrence_ws_bytes": (C.c_size_t, [_L, C.c_int, C.c_int, C.c_int]),
     "dssm_linear_recurrence": (C.c_int, [_P, _L, _L, _P, _L, _L, C.c_int, _P, _P, _L, C.c_int, C.c_int, C.c_int, _P, _L,

@@ -25,46 +25,46 @@ namespace seq {
 namespace {
 
 // ---- lookup ------------------------------------------------------------------------------------
-// A row takes G lanes of 8 columns each (G a power of two up to 64, wider rows loop), a wave 64 / G rows;
-// each lane has kLookRows rows' loads in flight, since a row is one dependent gather behind its id.
+// A lane owns V neighbouring columns (8, 4 or 1: the widest that divides E, so that every access is whole),
+// a row takes G lanes (a power of two up to 64, wider rows loop) and a wave 64 / G rows.  A row is one
+// dependent gather behind its id, so each lane has kLookRows rows in flight: the ids first, then the rows
+// as they are, converted only when all have been asked for.
 constexpr int kLookRows = 4;
 
-template <typename T, typename O, typename I>
+template <typename T, typename O, typename I, int V>
 __global__ __launch_bounds__(256) void k_lookup(const T* __restrict__ table, int64_t ldt, const I* __restrict__ ids,
-                                                int64_t n, int64_t V, int E, float scale, O* __restrict__ out,
+                                                int64_t n, int64_t words, int E, float scale, O* __restrict__ out,
                                                 int lg) {
   const int G = 1 << lg, slot = threadIdx.x >> lg, slots = 256 >> lg;
   const int64_t r0 = (int64_t)blockIdx.x * slots * kLookRows + slot;
-  for (int c = (threadIdx.x & (G - 1)) * 8; c < E; c += G * 8) {
-    const int nv = E - c;
-    float x[kLookRows][8];
-    bool in[kLookRows];
+  int64_t id[kLookRows];
 #pragma unroll
-    for (int j = 0; j < kLookRows; ++j) {
-      const int64_t r = r0 + (int64_t)j * slots;
-      const int64_t id = r < n ? (int64_t)ids[r] : -1;
-      in[j] = id >= 0 && id < V;
-      if (in[j]) {
-        ld_row<T, 8>(table + id * ldt + c, nv, x[j]);
-      } else {
+  for (int j = 0; j < kLookRows; ++j) {
+    const int64_t r = r0 + (int64_t)j * slots;
+    id[j] = r < n ? (int64_t)ids[r] : -1;
+  }
+  for (int c = (threadIdx.x & (G - 1)) * V; c < E; c += G * V) {
+    Pack<T, V> x[kLookRows];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
-      }
-    }
+    for (int j = 0; j < kLookRows; ++j)
+      if (id[j] >= 0 && id[j] < words) x[j] = ldv<T, V>(table + id[j] * ldt + c);
 #pragma unroll
     for (int j = 0; j < kLookRows; ++j) {
       const int64_t r = r0 + (int64_t)j * slots;
       if (r >= n) continue;
+      const bool in = id[j] >= 0 && id[j] < words;
+      Pack<O, V> y;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[j][i] = in[j] ? x[j][i] * scale : 0.f;
-      st_row<O, 8>(out + r * E + c, nv, x[j]);
+      for (int i = 0; i < V; ++i) y.v[i] = st1<O>(in ? ld1(x[j].v[i]) * scale : 0.f);
+      stv<O, V>(out + r * E + c, y);
     }
   }
 }
 
 // ---- sort --------------------------------------------------------------------------------------
-constexpr int kTile = 4096;     // pairs a workgroup ranks
-constexpr int kItems = 4;       // of them a thread's (1024 threads)
+// Pairs a workgroup of 1024 threads ranks: 1 or 4 a thread.  The ranking is what a pass spends its time on,
+// and it is the same instructions whether 48 or 192 compute units run them: one a thread until the tiles'
+// counts, which every workgroup reads, become the larger part (kOwnSums).
 constexpr int kMaxBins = 1024;  // digits of at most 10 bits
 
 struct Fill {  // the part of the gradient that a launch's extra workgroups clear
@@ -89,8 +89,9 @@ __device__ __forceinline__ unsigned key_of(const I* ids, int64_t i, unsigned V) 
 
 // Ranks a tile's pairs by digit, stably: hist[w][d] becomes the number of the tile's pairs of digit d in
 // waves before w, total[d] the tile's count, and rank[] each pair's place among its wave's pairs of its
-// digit.  Wave w holds the pairs [256 w, 256 w + 256), lane-major within each of the four items.  A
+// digit.  Wave w holds 64 kItems pairs in a row, lane-major within each item.  A
 // wave's lanes find the lanes of their own digit by one ballot per digit bit.  Every thread calls this.
+template <int kItems>
 __device__ __forceinline__ void rank_tile(const unsigned (&dig)[kItems], const bool (&live)[kItems], int bits,
                                           unsigned short (*hist)[kMaxBins], unsigned* total, int (&rank)[kItems]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << bits;
@@ -148,18 +149,21 @@ __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* s) {
 }
 
 struct SortLds {
-  unsigned short hist[16][kMaxBins];
+  __attribute__((aligned(16))) unsigned short hist[16][kMaxBins];
   unsigned total[kMaxBins];
   unsigned scan[16];
 };
 
-// The whole sort of one tile (n <= 4096) in one workgroup: the digits' passes move the pairs through LDS.
+// The whole sort of at most 4096 pairs in one workgroup: the digits' passes move the pairs through LDS.
+constexpr int kOneSort = 4096;
+
 template <typename I>
 __global__ __launch_bounds__(1024) void k_sort_one(const I* __restrict__ ids, int n, unsigned V, int bits, int passes,
-                                                   unsigned* __restrict__ key, int* __restrict__ pos, Fill f) {
+                                                   uint2* __restrict__ pairs, Fill f) {
+  constexpr int kItems = kOneSort / 1024;
   __shared__ SortLds s;
-  __shared__ unsigned lk[kTile];
-  __shared__ unsigned short lp[kTile];
+  __shared__ unsigned lk[kOneSort];
+  __shared__ unsigned short lp[kOneSort];
   if ((int)blockIdx.x >= f.first) return fill_role(f, blockIdx.x - f.first, gridDim.x - f.first);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   unsigned k[kItems];
@@ -167,7 +171,7 @@ __global__ __launch_bounds__(1024) void k_sort_one(const I* __restrict__ ids, in
   bool live[kItems];
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
-    const int i = w * 256 + j * 64 + lane;
+    const int i = w * 64 * kItems + j * 64 + lane;
     live[j] = i < n;
     k[j] = live[j] ? key_of(ids, i, V) : 0u;
     p[j] = i;
@@ -191,7 +195,7 @@ __global__ __launch_bounds__(1024) void k_sort_one(const I* __restrict__ ids, in
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kItems; ++j) {
-      const int i = w * 256 + j * 64 + lane;
+      const int i = w * 64 * kItems + j * 64 + lane;
       if (live[j]) {
         k[j] = lk[i];
         p[j] = lp[i];
@@ -201,19 +205,16 @@ __global__ __launch_bounds__(1024) void k_sort_one(const I* __restrict__ ids, in
   }
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
-    const int i = w * 256 + j * 64 + lane;
-    if (live[j]) {
-      key[i] = k[j];
-      pos[i] = p[j];
-    }
+    const int i = w * 64 * kItems + j * 64 + lane;
+    if (live[j]) pairs[i] = make_uint2(k[j], (unsigned)p[j]);
   }
 }
 
 // A pass over many tiles: counts per tile and digit (cnt [tiles x 1 << bits]) ...
-template <typename I>
-__global__ __launch_bounds__(1024) void k_sort_count(const I* __restrict__ ids, const unsigned* __restrict__ kin,
-                                                     int64_t n, unsigned V, int shift, int bits,
-                                                     unsigned* __restrict__ cnt, Fill f) {
+template <typename I, int kItems>
+__global__ __launch_bounds__(1024) void k_sort_count(const I* __restrict__ ids, const uint2* __restrict__ in, int64_t n,
+                                                     unsigned V, int shift, int bits, unsigned* __restrict__ cnt,
+                                                     Fill f) {
   __shared__ unsigned h[4][kMaxBins];  // four copies, so that a hot digit's adds do not all queue at one word
   if ((int)blockIdx.x >= f.first) return fill_role(f, blockIdx.x - f.first, gridDim.x - f.first);
   const int bins = 1 << bits;
@@ -221,9 +222,9 @@ __global__ __launch_bounds__(1024) void k_sort_count(const I* __restrict__ ids, 
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
-    const int64_t i = (int64_t)blockIdx.x * kTile + j * 1024 + threadIdx.x;
+    const int64_t i = (int64_t)blockIdx.x * 1024 * kItems + j * 1024 + threadIdx.x;
     if (i < n) {
-      const unsigned k = kin ? kin[i] : key_of(ids, i, V);
+      const unsigned k = in ? in[i].x : key_of(ids, i, V);
       atomicAdd(&h[threadIdx.x & 3][(k >> shift) & (bins - 1)], 1u);
     }
   }
@@ -262,11 +263,11 @@ __global__ __launch_bounds__(1024) void k_sort_sums(unsigned* __restrict__ cnt, 
 // ... and each tile's pairs to their places.  `summed`: cnt holds running sums (k_sort_sums); otherwise a
 // thread adds up its digit's counts itself, all tiles' for the digit's start and the earlier ones' for the
 // tile's place in it.
-template <typename I>
-__global__ __launch_bounds__(1024) void k_sort_place(const I* __restrict__ ids, const unsigned* __restrict__ kin,
-                                                     const int* __restrict__ pin, int64_t n, unsigned V, int shift,
-                                                     int bits, const unsigned* __restrict__ cnt, int tiles, int summed,
-                                                     unsigned* __restrict__ kout, int* __restrict__ pout, Fill f) {
+template <typename I, int kItems>
+__global__ __launch_bounds__(1024) void k_sort_place(const I* __restrict__ ids, const uint2* __restrict__ in, int64_t n,
+                                                     unsigned V, int shift, int bits,
+                                                     const unsigned* __restrict__ cnt, int tiles, int summed,
+                                                     uint2* __restrict__ out, Fill f) {
   __shared__ SortLds s;
   if ((int)blockIdx.x >= f.first) return fill_role(f, blockIdx.x - f.first, gridDim.x - f.first);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << bits, me = blockIdx.x;
@@ -275,36 +276,48 @@ __global__ __launch_bounds__(1024) void k_sort_place(const I* __restrict__ ids, 
   bool live[kItems];
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
-    const int64_t i = (int64_t)me * kTile + w * 256 + j * 64 + lane;
+    const int64_t i = (int64_t)me * 1024 * kItems + w * 64 * kItems + j * 64 + lane;
     live[j] = i < n;
-    k[j] = !live[j] ? 0u : kin ? kin[i] : key_of(ids, i, V);
-    p[j] = !live[j] ? 0 : kin ? pin[i] : (int)i;
+    uint2 kp = make_uint2(0u, (unsigned)i);
+    if (live[j] && in) kp = in[i];
+    else if (live[j]) kp.x = key_of(ids, i, V);
+    k[j] = kp.x;
+    p[j] = (int)kp.y;
     dig[j] = (k[j] >> shift) & (bins - 1);
   }
   unsigned all = 0, before = 0;
-  if ((int)threadIdx.x < bins) {
-    const unsigned* c = cnt + threadIdx.x;
-    if (summed) {
-      before = c[(int64_t)me * bins];
-      all = c[(int64_t)tiles * bins];
-    } else {
-      int t = 0;
-      for (; t + 16 <= tiles; t += 16) {
-        unsigned v[16];
+  if (summed) {
+    if ((int)threadIdx.x < bins) {
+      before = cnt[(int64_t)me * bins + threadIdx.x];
+      all = cnt[(int64_t)tiles * bins + threadIdx.x];
+    }
+  } else {
+    // a thread adds up four digits (one 16-byte load a tile) over every `share`th tile; the shares meet in
+    // LDS: share * bins = 4096 sums of each kind, the 32 KB of s.hist before it ranks
+    const int d4 = threadIdx.x & (bins / 4 - 1), q = threadIdx.x >> (bits - 2), share = 4096 >> bits;
+    uint4 a4 = make_uint4(0, 0, 0, 0), b4 = a4;
+    for (int t = q; t < tiles; t += 8 * share) {
+      uint4 v[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = c[(t + i) * bins];
+      for (int i = 0; i < 8; ++i)
+        if (t + i * share < tiles) v[i] = *reinterpret_cast<const uint4*>(cnt + (t + i * share) * bins + d4 * 4);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          all += v[i];
-          before += t + i < me ? v[i] : 0u;
-        }
-      }
-      for (; t < tiles; ++t) {
-        const unsigned v = c[t * bins];
-        all += v;
-        before += t < me ? v : 0u;
+      for (int i = 0; i < 8; ++i) {
+        const int at = t + i * share;
+        if (at < tiles) a4 = make_uint4(a4.x + v[i].x, a4.y + v[i].y, a4.z + v[i].z, a4.w + v[i].w);
+        if (at < min(tiles, me)) b4 = make_uint4(b4.x + v[i].x, b4.y + v[i].y, b4.z + v[i].z, b4.w + v[i].w);
       }
     }
+    unsigned* sum = reinterpret_cast<unsigned*>(s.hist);
+    *reinterpret_cast<uint4*>(sum + q * bins + d4 * 4) = a4;
+    *reinterpret_cast<uint4*>(sum + 4096 + q * bins + d4 * 4) = b4;
+    __syncthreads();
+    if ((int)threadIdx.x < bins)
+      for (int i = 0; i < share; ++i) {
+        all += sum[i * bins + threadIdx.x];
+        before += sum[4096 + i * bins + threadIdx.x];
+      }
+    __syncthreads();
   }
   rank_tile(dig, live, bits, s.hist, s.total, rank);
   const unsigned start = block_scan(all, s.scan) + before;
@@ -314,74 +327,103 @@ __global__ __launch_bounds__(1024) void k_sort_place(const I* __restrict__ ids, 
   for (int j = 0; j < kItems; ++j)
     if (live[j]) {
       const unsigned at = s.total[dig[j]] + s.hist[w][dig[j]] + rank[j];
-      kout[at] = k[j];
-      pout[at] = p[j];
+      out[at] = make_uint2(k[j], (unsigned)p[j]);
     }
 }
 
 // ---- sums --------------------------------------------------------------------------------------
-// Span s of the sorted list is [s S, (s + 1) S).  G lanes of 8 columns walk it, eight rows' loads in
-// flight.  part[2 s] takes the run that came in from span s - 1, part[2 s + 1] the run that goes on into
-// span s + 1 and starts in s; a run that fills a whole span and goes on both ways counts as incoming.
-constexpr int kSpan = 32;
+// A group of G lanes, V columns each, sums a stretch of kStretch entries of the sorted list, all rows in
+// flight at once; the workgroup's 256 / G stretches are its span.  A run of one token that lies inside a
+// stretch goes to the table at once; the pieces of a run that crosses stretches meet in LDS; one that
+// crosses spans leaves part[2 s] (the piece of span s that came in from span s - 1) and part[2 s + 1] (the
+// piece that starts in s and goes on) for k_grad_join.  A piece that fills its span counts as incoming.
+constexpr int kStretch = 8;
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_grad_spans(const unsigned* __restrict__ key, const int* __restrict__ pos,
-                                                    int64_t n, unsigned V, const T* __restrict__ dy, int64_t lddy,
-                                                    int E, float scale, float* __restrict__ dtable,
-                                                    float* __restrict__ part, int lg) {
-  const int G = 1 << lg;
-  const int64_t s = (int64_t)blockIdx.x * (256 >> lg) + (threadIdx.x >> lg);
-  const int64_t i0 = s * kSpan, i1 = min(i0 + kSpan, n);
-  if (i0 >= n) return;
+template <typename T, int V>
+__global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pairs, int64_t n, unsigned words,
+                                                    const T* __restrict__ dy, int64_t lddy, int E, float scale,
+                                                    float* __restrict__ dtable, float* __restrict__ part, int lg) {
+  __shared__ float came[V * 256], goes[V * 256];
+  __shared__ unsigned char flags[256];
+  enum { kOut = 1, kOne = 2 };  // the last run goes on into the next stretch; there is one run
+  const int G = 1 << lg, groups = 256 >> lg, g = threadIdx.x >> lg, lane = threadIdx.x & (G - 1);
+  const int64_t i0 = ((int64_t)blockIdx.x * groups + g) * kStretch, i1 = min(i0 + kStretch, n);
   const unsigned none = 0xffffffffu;
-  const unsigned prev = i0 ? key[i0 - 1] : none, next = i1 < n ? key[i1] : none;
-  for (int c = (threadIdx.x & (G - 1)) * 8; c < E; c += G * 8) {
-    const int nv = E - c;
-    float acc[8];
+  uint2 k[kStretch];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-    unsigned cur = key[i0];
-    bool incoming = cur == prev;
-    auto flush = [&](bool outgoing) {
-      if (cur >= V) return;
-      if (!incoming && !outgoing) {
-        float y[8];
+  for (int j = 0; j < kStretch; ++j) k[j] = i0 + j < n ? pairs[i0 + j] : make_uint2(none, 0u);
+  const unsigned prev = i0 && i0 < n ? pairs[i0 - 1].x : none, next = i1 < n ? pairs[i1].x : none;
+  unsigned last = k[0].x;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = acc[i] * scale;
-        st_row<float, 8>(dtable + (int64_t)cur * E + c, nv, y);
-      } else {
-        st_row<float, 8>(part + (2 * s + (incoming ? 0 : 1)) * E + c, nv, acc);
-      }
-    };
-    for (int64_t i = i0; i < i1; i += 8) {
-      unsigned k[8];
-      float x[8][8];
+  for (int j = 1; j < kStretch; ++j) last = k[j].x != none ? k[j].x : last;
+  const bool live = i0 < n, in = live && k[0].x == prev, out = live && last == next;
+  if (lane == 0) flags[g] = (out ? kOut : 0) | (k[0].x == last ? kOne : 0);
+  for (int c0 = 0; c0 < E; c0 += G * V) {
+    const int c = c0 + lane * V;
+    const bool mine = c < E;
+    Pack<T, V> x[kStretch];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        k[j] = i + j < i1 ? key[i + j] : none;
-        if (k[j] < V) {
-          ld_row<T, 8>(dy + (int64_t)pos[i + j] * lddy + c, nv, x[j]);
-        } else {
+    for (int j = 0; j < kStretch; ++j)
+      if (mine && k[j].x < words) x[j] = ldv<T, V>(dy + (int64_t)k[j].y * lddy + c);
+    float acc[V];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) x[j][q] = 0.f;
-        }
-      }
+    for (int q = 0; q < V; ++q) acc[q] = 0.f;
+    bool incoming = in;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (k[j] == none) break;
-        if (k[j] != cur) {
-          flush(false);
-          cur = k[j];
+    for (int j = 0; j < kStretch; ++j) {
+      const unsigned cur = k[j].x, after = j + 1 < kStretch ? k[j + 1 < kStretch ? j + 1 : j].x : none;
+      if (mine && cur < words) {
+#pragma unroll
+        for (int q = 0; q < V; ++q) acc[q] += ld1(x[j].v[q]);
+        if (after != cur) {  // the run's end in this stretch
+          const bool outgoing = after == none && out;
+          if (incoming || outgoing) {
+            float* to = incoming ? came : goes;
+#pragma unroll
+            for (int q = 0; q < V; ++q) to[q * 256 + threadIdx.x] = acc[q];
+          } else {
+            Pack<float, V> y;
+#pragma unroll
+            for (int q = 0; q < V; ++q) y.v[q] = acc[q] * scale;
+            stv<float, V>(dtable + (int64_t)cur * E + c, y);
+          }
+#pragma unroll
+          for (int q = 0; q < V; ++q) acc[q] = 0.f;
           incoming = false;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) acc[q] = 0.f;
         }
-#pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] += x[j][q];
       }
     }
-    flush(cur == next);
+    __syncthreads();
+    // Who joins a run's pieces: the group where it starts, or group 0 for the one that came into the span.
+    const bool starts = out && !(in && (flags[g] & kOne)) && last < words;
+    const bool enters = g == 0 && in && k[0].x < words;
+#pragma unroll
+    for (int role = 0; role < 2; ++role) {
+      if (!mine || !(role ? starts : enters)) continue;
+      const float* from = role ? goes : came;
+      float sum[V];
+#pragma unroll
+      for (int q = 0; q < V; ++q) sum[q] = from[q * 256 + threadIdx.x];
+      bool on = role || ((flags[0] & kOne) && out);  // the run reaches the next stretch
+      int j = g + 1;
+      for (; on && j < groups; ++j) {
+#pragma unroll
+        for (int q = 0; q < V; ++q) sum[q] += came[q * 256 + (j << lg) + lane];
+        on = (flags[j] & kOne) && (flags[j] & kOut);
+      }
+      if (role && !on) {
+        Pack<float, V> y;
+#pragma unroll
+        for (int q = 0; q < V; ++q) y.v[q] = sum[q] * scale;
+        stv<float, V>(dtable + (int64_t)last * E + c, y);
+      } else {
+        Pack<float, V> y;
+#pragma unroll
+        for (int q = 0; q < V; ++q) y.v[q] = sum[q];
+        stv<float, V>(part + (2 * (int64_t)blockIdx.x + role) * E + c, y);
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -390,148 +432,175 @@ __global__ __launch_bounds__(256) void k_grad_spans(const unsigned* __restrict__
 // stretches of it and join them through LDS, so that half a list of one token is no chain of loads.
 constexpr int kShort = 8;
 
-__global__ __launch_bounds__(256) void k_grad_join(const unsigned* __restrict__ key, int64_t n, int64_t spans,
-                                                   unsigned V, int E, float scale, const float* __restrict__ part,
+template <int V>
+__global__ __launch_bounds__(256) void k_grad_join(const uint2* __restrict__ pairs, int64_t n, int64_t spans, int S,
+                                                   unsigned words, int E, float scale, const float* __restrict__ part,
                                                    float* __restrict__ dtable, int lg) {
   const int G = 1 << lg, groups = 256 >> lg, grp = threadIdx.x >> lg, lane = threadIdx.x & (G - 1);
-  __shared__ float red[256 * 8];
+  __shared__ float red[256 * V];
   __shared__ int64_t longs[256];
   __shared__ int nlong;
   if (threadIdx.x == 0) nlong = 0;
   __syncthreads();
   const int64_t s = (int64_t)blockIdx.x * groups + grp;
-  const int64_t end = (s + 1) * kSpan;  // the next span's first entry
-  const unsigned cur = end < n ? key[end] : V;
-  // the run starts in s: its token is not also the one that came in and fills the span from its start
-  const bool head = cur < V && key[end - 1] == cur && (key[s * kSpan] != cur || s == 0 || key[s * kSpan - 1] != cur);
-  if (head) {
-    // the last span that the run reaches
-    int64_t last = s + 1;
-    while (last - s <= kShort && (last + 1) * kSpan < n && key[(last + 1) * kSpan] == cur) ++last;
-    if (last - s <= kShort) {
-      for (int c = lane * 8; c < E; c += G * 8) {
-        const int nv = E - c;
-        float acc[8], x[8];
-        ld_row<float, 8>(part + (2 * s + 1) * E + c, nv, acc);
-        for (int64_t t = s + 1; t <= last; ++t) {
-          ld_row<float, 8>(part + 2 * t * E + c, nv, x);
+  const int64_t end = (s + 1) * S;  // the next span's first entry
+  if (end < n) {
+    // all the keys that decide, asked for together: the span's ends, the entry in front of it, and the
+    // first entries of the next spans
+    const unsigned cur = pairs[end].x, tail = pairs[end - 1].x, head = pairs[s * S].x;
+    const unsigned front = s ? pairs[s * S - 1].x : 0xffffffffu;
+    unsigned ahead[kShort];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) acc[q] += x[q];
+    for (int j = 0; j < kShort; ++j) ahead[j] = (s + 2 + j) * S < n ? pairs[(s + 2 + j) * S].x : 0xffffffffu;
+    // the run starts in s: its token is not also the one that came in and fills the span from its start
+    if (cur < words && tail == cur && (head != cur || front != cur)) {
+      int more = 0;  // spans behind s + 1 that the run reaches
+#pragma unroll
+      for (int j = 0; j < kShort; ++j) more += more == j && ahead[j] == cur;
+      if (more < kShort) {
+        for (int c = lane * V; c < E; c += G * V) {
+          Pack<float, V> x[kShort + 1];
+          x[0] = ldv<float, V>(part + (2 * s + 1) * E + c);
+#pragma unroll
+          for (int j = 0; j < kShort; ++j)
+            if (j <= more) x[j + 1] = ldv<float, V>(part + 2 * (s + 1 + j) * E + c);
+          Pack<float, V> y = x[0];
+#pragma unroll
+          for (int j = 0; j < kShort; ++j)
+            if (j <= more) {
+#pragma unroll
+              for (int q = 0; q < V; ++q) y.v[q] += x[j + 1].v[q];
+            }
+#pragma unroll
+          for (int q = 0; q < V; ++q) y.v[q] *= scale;
+          stv<float, V>(dtable + (int64_t)cur * E + c, y);
         }
-#pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] *= scale;
-        st_row<float, 8>(dtable + (int64_t)cur * E + c, nv, acc);
+      } else if (lane == 0) {
+        longs[atomicAdd(&nlong, 1)] = s;
       }
-    } else if (lane == 0) {
-      longs[atomicAdd(&nlong, 1)] = s;
     }
   }
   __syncthreads();
   for (int j = 0; j < nlong; ++j) {
     const int64_t h = longs[j];
-    const unsigned tok = key[(h + 1) * kSpan];
-    // the run's last span: the last one whose first entry is still this token (the list is sorted)
+    const unsigned tok = pairs[(h + 1) * S].x;
+    // the run's last span: the last one whose first entry is still this token.  The list is sorted, so of 256
+    // probes at equal distances a first few are this token's, and the last of those bounds the next round.
     int64_t lo = h + 1, hi = spans - 1;
     while (lo < hi) {
-      const int64_t mid = (lo + hi + 1) / 2;
-      if (key[mid * kSpan] == tok) lo = mid;
-      else hi = mid - 1;
+      const int64_t gap = (hi - lo + 255) / 256, at = lo + (threadIdx.x + 1) * gap;
+      const int hit = __syncthreads_count(at <= hi && pairs[at * S].x == tok);
+      hi = min(hi, lo + (hit + 1) * gap - 1);
+      lo += hit * gap;
     }
     const int64_t cnt = lo - h, per = (cnt + groups - 1) / groups;
     const int64_t a = min(h + 1 + grp * per, lo + 1), b = min(a + per, lo + 1);
-    for (int c0 = 0; c0 < E; c0 += G * 8) {
-      const int c = c0 + lane * 8, nv = E - c;
-      float acc[8];
+    for (int c0 = 0; c0 < E; c0 += G * V) {
+      const int c = c0 + lane * V;
+      float acc[V];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) acc[q] = 0.f;
-      if (nv > 0) {
+      for (int q = 0; q < V; ++q) acc[q] = 0.f;
+      if (c < E) {
         int64_t t = a;
-        for (; t + 4 <= b; t += 4) {
-          float x[4][8];
+        for (; t + 8 <= b; t += 8) {
+          Pack<float, V> x[8];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) ld_row<float, 8>(part + 2 * (t + u) * E + c, nv, x[u]);
+          for (int u = 0; u < 8; ++u) x[u] = ldv<float, V>(part + 2 * (t + u) * E + c);
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
+          for (int u = 0; u < 8; ++u)
 #pragma unroll
-            for (int q = 0; q < 8; ++q) acc[q] += x[u][q];
+            for (int q = 0; q < V; ++q) acc[q] += x[u].v[q];
         }
         for (; t < b; ++t) {
-          float x[8];
-          ld_row<float, 8>(part + 2 * t * E + c, nv, x);
+          const Pack<float, V> x = ldv<float, V>(part + 2 * t * E + c);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) acc[q] += x[q];
+          for (int q = 0; q < V; ++q) acc[q] += x.v[q];
         }
       }
 #pragma unroll
-      for (int q = 0; q < 8; ++q) red[q * 256 + threadIdx.x] = acc[q];
+      for (int q = 0; q < V; ++q) red[q * 256 + threadIdx.x] = acc[q];
       __syncthreads();
-      if (grp == 0 && nv > 0) {
-        float x[8];
-        ld_row<float, 8>(part + (2 * h + 1) * E + c, nv, x);
+      if (grp == 0 && c < E) {
+        Pack<float, V> x = ldv<float, V>(part + (2 * h + 1) * E + c);
         for (int g = 0; g < groups; ++g)
 #pragma unroll
-          for (int q = 0; q < 8; ++q) x[q] += red[q * 256 + (g << lg) + lane];
+          for (int q = 0; q < V; ++q) x.v[q] += red[q * 256 + (g << lg) + lane];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) x[q] *= scale;
-        st_row<float, 8>(dtable + (int64_t)tok * E + c, nv, x);
+        for (int q = 0; q < V; ++q) x.v[q] *= scale;
+        stv<float, V>(dtable + (int64_t)tok * E + c, x);
       }
       __syncthreads();
     }
   }
 }
 
-int lanes_log2(int E) {  // log2 of the lanes a row takes: 8 columns each, at most a wave
+// Columns a lane owns: the widest of 8, 4 and 1 that divides a row, `most` at most.
+int cols_of(int E, int most) { return most >= 8 && E % 8 == 0 ? 8 : E % 4 == 0 ? 4 : 1; }
+template <typename F>
+void by_cols_of(int v, F&& f) {
+  if (v == 8) f(std::integral_constant<int, 8>{});
+  else if (v == 4) f(std::integral_constant<int, 4>{});
+  else f(std::integral_constant<int, 1>{});
+}
+int lanes_log2(int E, int v) {  // log2 of the lanes a row takes, at most a wave
   int lg = 0;
-  while (lg < 6 && (8 << lg) < E) ++lg;
+  while (lg < 6 && (v << lg) < E) ++lg;
   return lg;
 }
+// Lanes and columns of the summing launch, and the entries of its workgroups' spans.
+template <typename T>
+constexpr int kGradCols = sizeof(T) == 4 ? 4 : 8;
+int span_of(int E, int dtype) {
+  return (256 >> lanes_log2(E, cols_of(E, dtype == DSSM_F32 ? kGradCols<float> : kGradCols<u16>))) * kStretch;
+}
+
+// More counts (tiles x bins) than this have their sums made by a launch of their own (k_sort_sums); up to it
+// every workgroup of k_sort_place adds them up itself, 1024 of them at a time.
+constexpr int64_t kOwnSums = 64 * 1024;
 
 // Workspace of a gradient: pairs twice, the tiles' digit counts, the spans' partial rows.
 struct GradWs {
-  int bits, passes;
+  int bits, passes, S, items, summed;
   int64_t tiles, spans;
-  size_t key0, pos0, key1, pos1, cnt, part, bytes;
+  size_t pairs[2], cnt, part, bytes;
 };
-GradWs grad_ws(int64_t n, int64_t V, int E) {
+GradWs grad_ws(int64_t n, int64_t V, int E, int dtype) {
   GradWs g{};
   int bits = 1;
   while (((int64_t)1 << bits) <= V) ++bits;  // keys 0 .. V
   g.passes = (bits + 9) / 10;
-  g.bits = (bits + g.passes - 1) / g.passes;
-  g.tiles = (n + kTile - 1) / kTile;
-  g.spans = (n + kSpan - 1) / kSpan;
+  g.bits = std::max(2, (bits + g.passes - 1) / g.passes);
+  const int64_t t1 = (n + 1023) / 1024;
+  g.items = (t1 << g.bits) <= kOwnSums ? 1 : 4;
+  g.tiles = (n + 1024 * g.items - 1) / (1024 * g.items);
+  g.summed = (g.tiles << g.bits) > kOwnSums;
+  g.S = span_of(E, dtype);
+  g.spans = (n + g.S - 1) / g.S;
   size_t at = 0;
   auto take = [&](size_t b) {
     const size_t o = at;
     at += (b + 255) / 256 * 256;
     return o;
   };
-  g.key0 = take(4 * n);
-  g.pos0 = take(4 * n);
-  g.key1 = take(4 * n);
-  g.pos1 = take(4 * n);
+  g.pairs[0] = take(8 * n);
+  g.pairs[1] = take(g.passes > 1 && n > kOneSort ? 8 * n : 0);
   g.cnt = take(4 * (size_t)(g.tiles + 1) << g.bits);
   g.part = take((size_t)g.spans * 2 * E * 4);
   g.bytes = at;
   return g;
 }
 bool grad_dims_ok(int64_t n, int64_t V, int E) {
-  return n >= 0 && n < ((int64_t)1 << 31) - kTile && V > 0 && V < ((int64_t)1 << 30) && E > 0 && E <= (1 << 20);
+  return n >= 0 && n < ((int64_t)1 << 31) - 4096 && V > 0 && V < ((int64_t)1 << 30) && E > 0 && E <= (1 << 20);
 }
-
-// More tiles than this have their counts summed by a launch of their own: a workgroup's own sums read
-// tiles x bins counts, 16 loads in flight.
-constexpr int kOwnSums = 64;
 
 template <typename I>
 int run_grad(const void* dy, int dtype, int64_t lddy, const I* ids, int64_t n, int64_t V, int E, float scale, float* dtable,
              char* ws, hipStream_t s) {
-  const GradWs g = grad_ws(n, V, E);
-  unsigned* key[2] = {(unsigned*)(ws + g.key0), (unsigned*)(ws + g.key1)};
-  int* pos[2] = {(int*)(ws + g.pos0), (int*)(ws + g.pos1)};
+  const GradWs g = grad_ws(n, V, E, dtype);
+  uint2* pairs[2] = {(uint2*)(ws + g.pairs[0]), (uint2*)(ws + g.pairs[1])};
   unsigned* cnt = (unsigned*)(ws + g.cnt);
   float* part = (float*)(ws + g.part);
-  const bool one = n <= kTile;
+  const bool one = n <= kOneSort;
   // the table's zeros, an equal share to each of the sort's launches
   const int64_t total = V * E, all4 = total / 4;
   const int shares = one ? 1 : 2 * g.passes;
@@ -553,34 +622,47 @@ int run_grad(const void* dy, int dtype, int64_t lddy, const I* ids, int64_t n, i
     return seq_status(zero_bytes_async(dtable, (size_t)total * 4, s));
   } else if (one) {
     const Fill f = part_of(1, &grid);
-    hipLaunchKernelGGL(k_sort_one<I>, dim3(grid), dim3(1024), 0, s, ids, (int)n, (unsigned)V, g.bits, g.passes, key[0],
-                       pos[0], f);
+    hipLaunchKernelGGL(k_sort_one<I>, dim3(grid), dim3(1024), 0, s, ids, (int)n, (unsigned)V, g.bits, g.passes,
+                       pairs[0], f);
   } else {
-    const int tiles = (int)g.tiles, summed = tiles > kOwnSums;
+    const int tiles = (int)g.tiles;
     for (int q = 0; q < g.passes; ++q) {
-      const unsigned* kin = q ? key[side] : nullptr;
-      const int* pin = q ? pos[side] : nullptr;
+      const uint2* in = q ? pairs[side] : nullptr;
       if (q) side ^= 1;
-      Fill f = part_of(tiles, &grid);
-      hipLaunchKernelGGL(k_sort_count<I>, dim3(grid), dim3(1024), 0, s, ids, kin, n, (unsigned)V, q * g.bits, g.bits, cnt,
-                         f);
-      if (summed)
-        hipLaunchKernelGGL(k_sort_sums, dim3(((1 << g.bits) + 63) / 64), dim3(1024), 0, s, cnt, tiles, 1 << g.bits);
-      f = part_of(tiles, &grid);
-      hipLaunchKernelGGL(k_sort_place<I>, dim3(grid), dim3(1024), 0, s, ids, kin, pin, n, (unsigned)V, q * g.bits, g.bits,
-                         cnt, tiles, summed, key[side], pos[side], f);
+      auto pass = [&](auto items) {
+        constexpr int kItems = decltype(items)::value;
+        Fill f = part_of(tiles, &grid);
+        hipLaunchKernelGGL((k_sort_count<I, kItems>), dim3(grid), dim3(1024), 0, s, ids, in, n, (unsigned)V, q * g.bits,
+                           g.bits, cnt, f);
+        if (g.summed)
+          hipLaunchKernelGGL(k_sort_sums, dim3(((1 << g.bits) + 63) / 64), dim3(1024), 0, s, cnt, tiles, 1 << g.bits);
+        f = part_of(tiles, &grid);
+        hipLaunchKernelGGL((k_sort_place<I, kItems>), dim3(grid), dim3(1024), 0, s, ids, in, n, (unsigned)V, q * g.bits,
+                           g.bits, cnt, tiles, g.summed, pairs[side], f);
+      };
+      if (g.items == 1) pass(std::integral_constant<int, 1>{});
+      else pass(std::integral_constant<int, 4>{});
     }
   }
-  const int lg = lanes_log2(E), groups = 256 >> lg;
-  const unsigned blocks = (unsigned)((g.spans + groups - 1) / groups);
+  auto blocks_of = [&](int lg) { return dim3((unsigned)((g.spans + (256 >> lg) - 1) / (256 >> lg))); };
   by_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
-    hipLaunchKernelGGL(k_grad_spans<T>, dim3(blocks), dim3(256), 0, s, key[side], pos[side], n, (unsigned)V, (const T*)dy,
-                       lddy, E, scale, dtable, part, lg);
+    by_cols_of(cols_of(E, kGradCols<T>), [&](auto vec) {
+      constexpr int VEC = decltype(vec)::value;
+      if constexpr (VEC <= kGradCols<T>)
+        hipLaunchKernelGGL((k_grad_spans<T, VEC>), dim3((unsigned)g.spans), dim3(256), 0, s, pairs[side], n, (unsigned)V,
+                           (const T*)dy, lddy, E, scale, dtable, part, lanes_log2(E, VEC));
+    });
   });
-  if (g.spans > 1)
-    hipLaunchKernelGGL(k_grad_join, dim3(blocks), dim3(256), 0, s, key[side], n, g.spans, (unsigned)V, E, scale, part,
-                       dtable, lg);
+  if (g.spans > 1) {
+    const int v = cols_of(E, 4), lg = lanes_log2(E, v);
+    if (v == 4)
+      hipLaunchKernelGGL(k_grad_join<4>, blocks_of(lg), dim3(256), 0, s, pairs[side], n, g.spans, g.S, (unsigned)V, E, scale,
+                         part, dtable, lg);
+    else
+      hipLaunchKernelGGL(k_grad_join<1>, blocks_of(lg), dim3(256), 0, s, pairs[side], n, g.spans, g.S, (unsigned)V, E, scale,
+                         part, dtable, lg);
+  }
   return seq_status(hipGetLastError());
 }
 
@@ -596,26 +678,29 @@ extern "C" int dssm_embedding_lookup(const void* table, int dtype, int64_t ldt, 
       (n > 0 && (!ids || !out)))
     return dssm::report_error(DSSM_E_INVALID, "embedding_lookup: bad argument");
   if (n == 0) return DSSM_OK;
-  const int lg = lanes_log2(E);
+  const int v = cols_of(E, 8), lg = lanes_log2(E, v);
   const int64_t rows = (int64_t)(256 >> lg) * kLookRows, blocks = (n + rows - 1) / rows;
   if (blocks > 0x7fffffff) return dssm::report_error(DSSM_E_UNSUPPORTED, "embedding_lookup: too many ids");
   by_dtype(dtype, [&](auto t) {
     by_dtype(out_dtype, [&](auto o) {
-      using T = decltype(t);
-      using O = decltype(o);
-      if (ids64)
-        hipLaunchKernelGGL((k_lookup<T, O, int64_t>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
-                           (const T*)table, ldt, (const int64_t*)ids, n, V, E, scale, (O*)out, lg);
-      else
-        hipLaunchKernelGGL((k_lookup<T, O, int32_t>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
-                           (const T*)table, ldt, (const int32_t*)ids, n, V, E, scale, (O*)out, lg);
+      by_cols_of(v, [&](auto vec) {
+        using T = decltype(t);
+        using O = decltype(o);
+        constexpr int VEC = decltype(vec)::value;
+        if (ids64)
+          hipLaunchKernelGGL((k_lookup<T, O, int64_t, VEC>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
+                             (const T*)table, ldt, (const int64_t*)ids, n, V, E, scale, (O*)out, lg);
+        else
+          hipLaunchKernelGGL((k_lookup<T, O, int32_t, VEC>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
+                             (const T*)table, ldt, (const int32_t*)ids, n, V, E, scale, (O*)out, lg);
+      });
     });
   });
   return seq_status(hipGetLastError());
 }
 
-extern "C" size_t dssm_embedding_grad_ws_bytes(int64_t n, int64_t V, int E) {
-  return grad_dims_ok(n, V, E) ? grad_ws(n, V, E).bytes + 256 : 0;
+extern "C" size_t dssm_embedding_grad_ws_bytes(int64_t n, int64_t V, int E, int dtype) {
+  return grad_dims_ok(n, V, E) && seq_dtype(dtype) ? grad_ws(n, V, E, dtype).bytes + 256 : 0;
 }
 
 extern "C" int dssm_embedding_grad(const void* dy, int dtype, int64_t lddy, const void* ids, int ids64, int64_t n,
@@ -624,7 +709,7 @@ extern "C" int dssm_embedding_grad(const void* dy, int dtype, int64_t lddy, cons
     return dssm::report_error(DSSM_E_INVALID, "embedding_grad: bad argument");
   if ((uintptr_t)dtable % 16 || (uintptr_t)ws % 16)
     return dssm::report_error(DSSM_E_INVALID, "embedding_grad: the gradient and the workspace are 16-byte aligned");
-  if (n > 0 && ws_bytes < grad_ws(n, V, E).bytes)
+  if (n > 0 && ws_bytes < grad_ws(n, V, E, dtype).bytes)
     return dssm::report_error(DSSM_E_INVALID, "embedding_grad: workspace too small (dssm_embedding_grad_ws_bytes)");
   return ids64 ? run_grad(dy, dtype, lddy, (const int64_t*)ids, n, V, E, scale, dtable, (char*)ws, (hipStream_t)stream)
                : run_grad(dy, dtype, lddy, (const int32_t*)ids, n, V, E, scale, dtable, (char*)ws, (hipStream_t)stream);

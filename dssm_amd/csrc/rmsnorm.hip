@@ -23,22 +23,41 @@ namespace {
 
 constexpr int kMaxCols = 16384;  // 1024 threads x 8 columns x 2
 
-// the sum of v over the NT threads that share a row (every thread gets it); s: one float a wave
-template <int NT>
-__device__ __forceinline__ float row_sum(float v, float* s) {
-  v = wave_allsum_step<0>(v);
-  v = wave_allsum_step<1>(v);
-  v = wave_allsum_step<2>(v);
-  v = wave_allsum_step<3>(v);
-  if constexpr (NT >= 64) {
-    v = wave_allsum_step<4>(v);
-    v = wave_allsum_step<5>(v);
+// the sum of v over the NT threads that share a row (every thread gets it); s: one value a wave
+__device__ __forceinline__ double dpp_add(double v, int stage) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const int lo = (int)(unsigned)u, hi = (int)(u >> 32);
+  int a, b;
+  if (stage == 0) {
+    a = __builtin_amdgcn_update_dpp(0, lo, 0xB1, 0xF, 0xF, false);
+    b = __builtin_amdgcn_update_dpp(0, hi, 0xB1, 0xF, 0xF, false);
+  } else if (stage == 1) {
+    a = __builtin_amdgcn_update_dpp(0, lo, 0x4E, 0xF, 0xF, false);
+    b = __builtin_amdgcn_update_dpp(0, hi, 0x4E, 0xF, 0xF, false);
+  } else if (stage == 2) {
+    a = __builtin_amdgcn_update_dpp(0, lo, 0x141, 0xF, 0xF, false);
+    b = __builtin_amdgcn_update_dpp(0, hi, 0x141, 0xF, 0xF, false);
+  } else {
+    a = __builtin_amdgcn_update_dpp(0, lo, 0x140, 0xF, 0xF, false);
+    b = __builtin_amdgcn_update_dpp(0, hi, 0x140, 0xF, 0xF, false);
   }
+  return v + __builtin_bit_cast(double, (unsigned long long)(unsigned)a | ((unsigned long long)(unsigned)b << 32));
+}
+__device__ __forceinline__ float dpp_add(float v, int stage) {
+  return stage == 0 ? wave_allsum_step<0>(v) : stage == 1 ? wave_allsum_step<1>(v) : stage == 2 ? wave_allsum_step<2>(v)
+                                                                                              : wave_allsum_step<3>(v);
+}
+template <int NT, typename F>
+__device__ __forceinline__ F row_sum(F v, F* s) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v = dpp_add(v, k);
+  if constexpr (NT >= 32) v = sum_xor16(v);
+  if constexpr (NT >= 64) v = sum_xor32(v);
   if constexpr (NT > 64) {
     const int w = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) s[w] = v;
     __syncthreads();
-    v = 0.f;
+    v = 0;
 #pragma unroll
     for (int i = 0; i < NT / 64; ++i) v += s[i];
     __syncthreads();
@@ -60,62 +79,85 @@ struct NormArgs {
   float eps;
 };
 
-// MODE 0: y in T; 1: y in the 8-bit form; 2: x itself in the 8-bit form (no norm)
+// MODE 0: y in T; 1: y in the 8-bit form; 2: x itself in the 8-bit form (no norm).
+// A workgroup walks rows blockIdx.x * kRows + i * gridDim.x * kRows with the weights in registers and the next
+// rows' loads in flight behind the current ones' arithmetic.
 template <typename T, int NT, int K, int MODE>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
   constexpr int kRows = NT < 256 ? 256 / NT : 1;
-  __shared__ float red[16];
+  __shared__ double red[16];
   const int l = threadIdx.x % NT;
-  const int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / NT;
-  const bool in = r < a.rows;
-  float v[K][8];
-  float sum = 0.f;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  float w[K][8];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (k * NT + l) * 8, nv = a.cols - c;
-    if (in && nv > 0) {
-      ld_row<T, 8>((const T*)a.x + r * a.ldx + c, nv, v[k]);
+    if (MODE != 2 && nv > 0) ld_row<float, 8>(a.w + c, nv, w[k]);
+  }
+  Ask<T> x[K], b[K];
+  auto ask = [&](int64_t r) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * NT + l) * 8, nv = r < a.rows ? a.cols - c : 0;
+      x[k].ask((const T*)a.x + r * a.ldx + c, nv);
+      if (MODE != 2 && a.res) b[k].ask((const T*)a.res + r * a.ldres + c, nv);
+    }
+  };
+  int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / NT;
+  ask(r);
+  // (the loop's condition is the workgroup's, not the row slot's: its barriers need every thread)
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < a.rows; r0 += step, r += step) {
+    const bool in = r < a.rows;
+    float v[K][8], sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
+      x[k].take((const T*)a.x + r * a.ldx + c, nv, v[k]);
       if (MODE != 2 && a.res) {
-        float b[8];
-        ld_row<T, 8>((const T*)a.res + r * a.ldres + c, nv, b);
+        float t[8];
+        b[k].take((const T*)a.res + r * a.ldres + c, nv, t);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[k][i] = ld1(st1<T>(v[k][i] + b[i]));
+        for (int i = 0; i < 8; ++i) v[k][i] = ld1(st1<T>(v[k][i] + t[i]));
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
     }
+    ask(r + step);
     if constexpr (MODE != 2) {
-      if (in && nv > 0 && a.s) st_row<T, 8>((T*)a.s + r * a.lds + c, nv, v[k]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(v[k][i], v[k][i], sum);
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
+        if (a.s && nv > 0) st_row<T, 8>((T*)a.s + r * a.lds + c, nv, v[k]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fmaf(v[k][i], v[k][i], sum);
+      }
+      // A thread's squares in fp32, the row's in 64 bits: what a row's values share costs them no accuracy.
+      const double root = 1.0 / sqrt(row_sum<NT, double>((double)sum, red) / (double)a.cols + (double)a.eps);
+      const float rstd = (float)root, rest = (float)(root - (double)rstd);
+      if (in && l == 0 && a.rstd) a.rstd[r] = rstd;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          // v rstd w with the product's rounding error and rstd's rest put back: a value next to a border of
+          // the 8-bit grid falls to the side that it is on
+          const float p = v[k][i] * w[k][i], e = fmaf(v[k][i], w[k][i], -p);
+          v[k][i] = i < nv ? fmaf(p, rstd, fmaf(p, rest, e * rstd)) : 0.f;
+        }
+        if (MODE == 0 && nv > 0) st_row<T, 8>((T*)a.y + r * a.ldy + c, nv, v[k]);
+      }
     }
-  }
-  if constexpr (MODE != 2) {
-    const float rstd = 1.0f / sqrtf(row_sum<NT>(sum, red) / (float)a.cols + a.eps);
-    if (in && l == 0 && a.rstd) a.rstd[r] = rstd;
+    if constexpr (MODE != 0) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * NT + l) * 8, nv = a.cols - c;
-      if (nv <= 0) continue;
-      float w[8];
-      ld_row<float, 8>(a.w + c, nv, w);
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * NT + l) * 8;
+        float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[k][i] = i < nv ? v[k][i] * rstd * w[i] : 0.f;  // the form's padding is zero
-      if (MODE == 0 && in) st_row<T, 8>((T*)a.y + r * a.ldy + c, nv, v[k]);
-    }
-  }
-  if constexpr (MODE != 0) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * NT + l) * 8;
-      float m = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(v[k][i]));
-      const unsigned e = blk_exp(max16(m));
-      if (in && c < a.kp) {
-        *reinterpret_cast<uint2*>(a.q + r * a.kp + c) = to_e4m3x8(v[k], exp_inv(e));
-        if ((l & 15) == 0) a.scale[r * (a.kp / kBlk) + c / kBlk] = (unsigned char)e;
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(v[k][i]));
+        const unsigned e = blk_exp(max16(m));
+        if (in && c < a.kp) {
+          *reinterpret_cast<uint2*>(a.q + r * a.kp + c) = to_e4m3x8(v[k], exp_inv(e));
+          if ((l & 15) == 0) a.scale[r * (a.kp / kBlk) + c / kBlk] = (unsigned char)e;
+        }
       }
     }
   }
@@ -142,45 +184,54 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_bwd(NormArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[k][i] = 0.f;
   }
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < a.rows; r0 += (int64_t)gridDim.x * kRows) {
-    const int64_t r = r0 + g;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  Ask<T> as[K], ad[K], ax[K];
+  float arstd = 0.f;
+  auto ask = [&](int64_t r) {
     const bool in = r < a.rows;
-    const float rstd = in ? a.rstd_in[r] : 0.f;
-    float n[K][8], d[K][8], sum = 0.f;
+    if (in) arstd = a.rstd_in[r];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = (k * NT + l) * 8, nv = a.cols - c;
-      if (in && nv > 0) {
-        ld_row<T, 8>((const T*)a.s_in + r * a.lds + c, nv, n[k]);
-        ld_row<T, 8>((const T*)a.dy + r * a.lddy + c, nv, d[k]);
-      } else {
+      const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
+      as[k].ask((const T*)a.s_in + r * a.lds + c, nv);
+      ad[k].ask((const T*)a.dy + r * a.lddy + c, nv);
+      if (a.ds) ax[k].ask((const T*)a.ds + r * a.ldds + c, nv);
+    }
+  };
+  int64_t r = (int64_t)blockIdx.x * kRows + g;
+  ask(r);
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < a.rows; r0 += step, r += step) {
+    const bool in = r < a.rows;
+    const float rstd = arstd;
+    float n[K][8], d[K][8], o[K][8], sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) n[k][i] = d[k][i] = 0.f;
-      }
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
+      as[k].take((const T*)a.s_in + r * a.lds + c, nv, n[k]);
+      ad[k].take((const T*)a.dy + r * a.lddy + c, nv, d[k]);
+      if (a.ds) ax[k].take((const T*)a.ds + r * a.ldds + c, nv, o[k]);
+      else
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[k][i] = 0.f;
+    }
+    // (the tails of an element-by-element read are in hand here too: dx may be dy or ds)
+    ask(r + step);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        n[k][i] *= rstd;
+        n[k][i] = in ? n[k][i] * rstd : 0.f;
         dw[k][i] = fmaf(d[k][i], n[k][i], dw[k][i]);
         d[k][i] *= w[k][i];
         sum = fmaf(d[k][i], n[k][i], sum);
       }
-    }
-    const float mean = row_sum<NT>(sum, red) / (float)a.cols;
-    if (!in) continue;
+    const float mean = row_sum<NT, float>(sum, red) / (float)a.cols;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = (k * NT + l) * 8, nv = a.cols - c;
-      if (nv <= 0) continue;
-      float o[8];
+      const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = rstd * (d[k][i] - n[k][i] * mean);
-      if (a.ds) {
-        float b[8];
-        ld_row<T, 8>((const T*)a.ds + r * a.ldds + c, nv, b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] += b[i];
-      }
-      st_row<T, 8>((T*)a.dx + r * a.lddx + c, nv, o);
+      for (int i = 0; i < 8; ++i) o[k][i] = fmaf(rstd, d[k][i] - n[k][i] * mean, o[k][i]);
+      if (nv > 0) st_row<T, 8>((T*)a.dx + r * a.lddx + c, nv, o[k]);
     }
   }
   float* out = a.part + (int64_t)blockIdx.x * a.cols;
@@ -258,6 +309,7 @@ template <typename F>
 void by_cols(int cols, F&& f) {
   using std::integral_constant;
   if (cols <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else if (cols <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
   else if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
   else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
   else if (cols <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
@@ -277,14 +329,14 @@ void run_norm(const NormArgs& a, int dtype, hipStream_t s) {
     using T = decltype(tag);
     by_cols(a.cols, [&](auto nt, auto kk) {
       constexpr int NT = decltype(nt)::value, K = decltype(kk)::value, rows = NT < 256 ? 256 / NT : 1;
-      hipLaunchKernelGGL((k_norm<T, NT, K, MODE>), dim3((unsigned)((a.rows + rows - 1) / rows)),
-                         dim3(NT < 256 ? 256 : NT), 0, s, a);
+      const int64_t blocks = std::min<int64_t>((a.rows + rows - 1) / rows, NT < 1024 ? 2048 : 512);
+      hipLaunchKernelGGL((k_norm<T, NT, K, MODE>), dim3((unsigned)blocks), dim3(NT < 256 ? 256 : NT), 0, s, a);
     });
   });
 }
 constexpr int kBwdBlocks = 1024;  // partial rows of dw at most
 int bwd_blocks(int64_t rows, int cols) {
-  const int per = cols <= 128 ? 16 : cols <= 1024 ? 4 : 1;  // rows a workgroup takes at once
+  const int per = cols <= 128 ? 16 : cols <= 256 ? 8 : cols <= 1024 ? 4 : 1;  // rows a workgroup takes at once
   return (int)std::max<int64_t>(1, std::min<int64_t>(kBwdBlocks, (rows + per - 1) / per));
 }
 

@@ -68,6 +68,26 @@ __device__ __forceinline__ void st_row(T* p, int n, const float (&x)[V]) {
   }
 }
 
+// The same load in two steps, so that a kernel asks for all it needs before it waits for any: ask() issues a
+// whole group's access and does not look at it, take() converts (a ragged group is read element by element
+// there: only the last lane of a row whose width is no multiple of 8 has one).
+template <typename T>
+struct Ask {
+  Pack<T, 8> r;
+  __device__ __forceinline__ void ask(const T* p, int n) {
+    if (n >= 8) r = ldv<T, 8>(p);
+  }
+  __device__ __forceinline__ void take(const T* p, int n, float (&x)[8]) const {
+    if (n >= 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = ld1(r.v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = i < n ? ld1(p[i]) : 0.f;
+    }
+  }
+};
+
 // ---- the 8-bit block form ---------------------------------------------------------------------------
 // A row's 128 columns share the power of two 2^e, the smallest that brings their largest finite
 // magnitude into e4m3's +-448; it is stored as the byte e + 127 (E8M0), which the matrix instruction

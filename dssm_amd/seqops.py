@@ -47,19 +47,25 @@ def _code(dtype: torch.dtype, what: str) -> int:
 
 
 def _on_gpu(first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
-    dev = first.device
+    dev = first.get_device()  # (-1: host memory)
     for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-    if dev.type != "cuda":
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    if dev < 0:
         raise ValueError("tensors must be on the GPU (the HIP path has no CPU fallback)")
-    return dev
+    return first.device
+
+
+_entries = {}
 
 
 def _call(dev: torch.device, name: str, *args):
     """The entry point on the device's current stream, with that device current."""
-    f = getattr(_lib.load(), name)
-    stream = torch.cuda.current_stream(dev).cuda_stream
+    f = _entries.get(name)
+    if f is None:
+        f = _entries[name] = getattr(_lib.load(), name)
+    # the handle itself: the wrapper object of torch.cuda.current_stream() costs as much as half a launch
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
     if dev.index == torch.cuda.current_device():
         rc = f(*args, stream)
     else:
@@ -125,7 +131,7 @@ def embedding_grad(dy: torch.Tensor, ids: torch.Tensor, nwords: int, scale: floa
         raise ValueError("dy must be [*ids.shape, E]")
     V, E, n = int(nwords), dy.shape[-1], ids.numel()
     lib = _lib.load()
-    need = int(lib.dssm_embedding_grad_ws_bytes(n, V, E))
+    need = int(lib.dssm_embedding_grad_ws_bytes(n, V, E, code))
     if not need:
         raise ValueError(f"embedding_grad: {n} ids, {V} words, {E} columns are out of range "
                          "(fewer than 2^31 - 4096 ids, 1 to 2^30 - 1 words, 1 to 2^20 columns)")

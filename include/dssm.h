@@ -705,7 +705,7 @@ int dssm_embedding_lookup(const void* table, int dtype, int64_t ldt, int64_t V, 
  * summed by token, in the order of their positions (the result does not depend on timing); ids outside
  * [0, V) are left out.  n < 2^31 - 4096, V < 2^30, E <= 2^20.  ws: dssm_embedding_grad_ws_bytes() bytes,
  * 16-byte aligned, of any content (0: a size is out of range). */
-size_t dssm_embedding_grad_ws_bytes(int64_t n, int64_t V, int E);
+size_t dssm_embedding_grad_ws_bytes(int64_t n, int64_t V, int E, int dtype);
 int dssm_embedding_grad(const void* dy, int dtype, int64_t lddy, const void* ids, int ids64, int64_t n, int64_t V, int E,
                         float scale, float* dtable, void* ws, size_t ws_bytes, void* stream);
 

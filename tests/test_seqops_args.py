@@ -106,7 +106,7 @@ def test_c_entries_refuse():
     ]
     assert bad == [-1] * len(bad)
     assert lib.dssm_last_error()
-    assert lib.dssm_embedding_grad_ws_bytes(1 << 31, 4, 4) == 0
+    assert lib.dssm_embedding_grad_ws_bytes(1 << 31, 4, 4, L) == 0
     assert lib.dssm_rms_norm_bwd_ws_bytes(4, 16385) == 0
 
 
