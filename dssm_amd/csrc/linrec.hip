@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "seq.h"
 
@@ -35,15 +36,19 @@ namespace {
 
 constexpr int kPiece = DSSM_RECUR_PIECE;
 
-// u = sigmoid(f) and v = 1 - u, both to fp32 accuracy: e = exp(-|f|) never overflows and neither result
-// is a difference.  exp(x) = 2^(x log2 e) with the product's rounding error and log2 e's own put back
-// (the hardware's 2^x alone would be off by |x| roundings).
+// u = sigmoid(f) and v = 1 - u, neither a difference: e = exp(-|f|) never overflows, and whichever of u and v
+// is small keeps its relative accuracy.  The hardware's 2^x is off by the rounding of its argument, |x| half
+// units: for fp32 gates that rounding and log2 e's own are put back, for gates that were rounded to 16 bits
+// (whose own half step moves e by |x| 2^-12 and more) they are not.
+template <typename T>
 __device__ __forceinline__ void gate_uv(float f, float& u, float& v) {
-  const float x = -fabsf(f), kL = 1.44269502f, kLlo = 1.92596303e-8f;
-  const float hi = x * kL, lo = fmaf(x, kL, -hi) + x * kLlo;
+  const float kL = 1.44269502f, kLlo = 1.92596303e-8f;
+  const float hi = -fabsf(f) * kL;
   float e = __builtin_amdgcn_exp2f(hi);
-  e = fmaf(e, lo * 0.693147182f, e);
-  e = x > -126.f * 0.69f ? e : (x == x ? 0.f : x);  // (-inf would give inf - inf)
+  if constexpr (sizeof(T) == 4) {
+    const float x = -fabsf(f), lo = fmaf(x, kL, -hi) + x * kLlo;
+    e = hi < -126.f ? 0.f : fmaf(e, lo * 0.693147182f, e);  // (-inf would give inf - inf; NaN stays)
+  }
   const float r = __builtin_amdgcn_rcpf(1.f + e), q = e * r;
   u = f >= 0.f ? r : q;
   v = f >= 0.f ? q : r;
@@ -67,7 +72,7 @@ struct RecurArgs {
 
 template <int V>
 struct Unit {  // a lane's channels
-  int64_t r, ch;  // row, first channel in [R x H]
+  int64_t r, r0, ch;  // row, the wave's first row, first channel in [R x H]
   int c, lo, hi;  // column; active steps [lo, hi) in walking order
   bool in;
 };
@@ -75,7 +80,7 @@ template <int V>
 __device__ __forceinline__ Unit<V> unit_of(const RecurArgs& a, int64_t u) {
   Unit<V> t;
   t.in = u < a.R * a.upr;
-  if (!t.in) u = 0;
+  if (!t.in) u = a.R * a.upr - 1;
   t.r = u / a.upr;
   t.c = (int)(u - t.r * a.upr) * V;
   t.ch = t.r * a.H + t.c;
@@ -84,39 +89,75 @@ __device__ __forceinline__ Unit<V> unit_of(const RecurArgs& a, int64_t u) {
   if (!t.in) len = 0;
   t.lo = a.reverse ? a.T - len : 0;
   t.hi = a.reverse ? a.T : len;
+  const int64_t r0 = t.r;  // (rows do not fall from lane to lane: the first lane's is the wave's smallest)
+  t.r0 = ((int64_t)__builtin_amdgcn_readfirstlane((int)(r0 >> 32)) << 32) |
+         (unsigned)__builtin_amdgcn_readfirstlane((int)r0);
   return t;
 }
-// element pointer of the unit at walking step 0, and the walking stride
-template <typename T>
-__device__ __forceinline__ T* walk(T* p, const RecurArgs& a, int64_t sr, int64_t st, int64_t r, int c) {
-  return p + r * sr + c + (a.reverse ? (int64_t)(a.T - 1) * st : 0);
-}
+// A tensor as a wave walks it: the address of walking step p is uniform + the lane's offset, which is a
+// 32-bit one behind the wave's first row where the rows of a wave lie close enough (W false: any strides),
+// so that sixteen loads in flight hold one offset register and not sixteen addresses.
+template <typename T, bool W>
+struct Walk {
+  char* base;
+  int64_t step;
+  std::conditional_t<W, int64_t, unsigned> off;
+  __device__ __forceinline__ Walk(const void* p, const RecurArgs& a, int64_t sr, int64_t st, int64_t r0, int64_t r, int c) {
+    base = (char*)p + (r0 * sr + (a.reverse ? (int64_t)(a.T - 1) * st : 0)) * (int64_t)sizeof(T);
+    step = (a.reverse ? -st : st) * (int64_t)sizeof(T);
+    off = (decltype(off))(((r - r0) * sr + c) * (int64_t)sizeof(T));
+  }
+  __device__ __forceinline__ T* at(int p) const { return (T*)(base + p * step + off); }
+};
 
-// A piece's u and x = (1 - u) cand; steps that do not act are u = 1, x = 0.
-template <typename T, int V>
-__device__ __forceinline__ void load_piece(const T* g, int64_t gs, const T* c, int64_t cs, int q0, int lo, int hi,
-                                           float (&u)[kPiece][V], float (&x)[kPiece][V]) {
+// A piece's gates and candidates as they lie in memory.  A step that does not act is not read; where all of
+// a wave's steps act, which most pieces are, nothing is compared.
+template <typename T, int V, bool W>
+struct Piece {
   Pack<T, V> a[kPiece], b[kPiece];
+  bool full;
+  __device__ __forceinline__ void ask(const Walk<T, W>& g, const Walk<T, W>& c, int q0, int lo, int hi) {
+    full = __all(q0 >= lo && q0 + kPiece <= hi);
+    if (full) {
 #pragma unroll
-  for (int i = 0; i < kPiece; ++i) {
-    const int p = q0 + i;
-    if (p >= lo && p < hi) {
-      a[i] = ldv<T, V>(g + p * gs);
-      b[i] = ldv<T, V>(c + p * cs);
+      for (int i = 0; i < kPiece; ++i) {
+        a[i] = ldv<T, V>(g.at(q0 + i));
+        b[i] = ldv<T, V>(c.at(q0 + i));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) {
+        const int p = q0 + i;
+        if (p >= lo && p < hi) {
+          a[i] = ldv<T, V>(g.at(p));
+          b[i] = ldv<T, V>(c.at(p));
+        }
+      }
     }
   }
+  // u and x = (1 - u) cand; steps that do not act are u = 1, x = 0
+  __device__ __forceinline__ void take(int q0, int lo, int hi, float (&u)[kPiece][V], float (&x)[kPiece][V]) const {
 #pragma unroll
-  for (int i = 0; i < kPiece; ++i) {
-    const bool on = q0 + i >= lo && q0 + i < hi;
+    for (int i = 0; i < kPiece; ++i)
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      float uu, vv;
-      gate_uv(ld1(a[i].v[k]), uu, vv);
-      u[i][k] = on ? uu : 1.f;
-      x[i][k] = on ? vv * ld1(b[i].v[k]) : 0.f;
+      for (int k = 0; k < V; ++k) {
+        float vv;
+        gate_uv<T>(ld1(a[i].v[k]), u[i][k], vv);
+        x[i][k] = vv * ld1(b[i].v[k]);
+      }
+    if (!full) {
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) {
+        const bool on = q0 + i >= lo && q0 + i < hi;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          u[i][k] = on ? u[i][k] : 1.f;
+          x[i][k] = on ? x[i][k] : 0.f;
+        }
+      }
     }
   }
-}
+};
 
 // The value that enters a segment: `start` carried through the earlier segments' maps.  The waves fold a
 // share of the segments each and join through LDS.  dir > 0: segments 0 .. s - 1; dir < 0: S - 1 .. s + 1.
@@ -157,31 +198,33 @@ __device__ __forceinline__ void enter_segment(const RecurArgs& a, const Unit<V>&
 
 // ---- forward -----------------------------------------------------------------------------------
 // SUM: only the segment's (A, B).
-template <typename T, int V, int NW, bool SUM>
+template <typename T, int V, int NW, bool SUM, bool W>
 __global__ __launch_bounds__(NW * 64) void k_recur_fwd(RecurArgs a) {
   __shared__ float lds[2][NW][64][2 * V];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // the replay walks the segments from the last: what the summing launch read last is what caches hold
   const int s = SUM ? (int)blockIdx.y : a.S - 1 - (int)blockIdx.y;
   const Unit<V> t = unit_of<V>(a, (int64_t)blockIdx.x * 64 + lane);
-  const int64_t gs = a.reverse ? -a.gt : a.gt, cs = a.reverse ? -a.ct : a.ct, hs = a.reverse ? -a.ht : a.ht;
-  const T* g = walk((const T*)a.gate, a, a.gr, a.gt, t.r, t.c);
-  const T* c = walk((const T*)a.cand, a, a.cr, a.ct, t.r, t.c);
-  T* ho = walk((T*)a.h, a, a.hr, a.ht, t.r, t.c);
+  const Walk<T, W> g(a.gate, a, a.gr, a.gt, t.r0, t.r, t.c), c(a.cand, a, a.cr, a.ct, t.r0, t.r, t.c);
+  const Walk<T, W> ho(a.h, a, a.hr, a.ht, t.r0, t.r, t.c);
   float carry[V], span[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     carry[k] = !SUM && a.h0 && t.in ? a.h0[t.ch + k] : 0.f;
     span[k] = 1.f;
   }
+  Piece<T, V, W> in;
+  in.ask(g, c, s * a.L + w * kPiece, t.lo, min(t.hi, min(s * a.L + a.L, a.T)));
   if constexpr (!SUM && NW > 1)
     if (a.S > 1) enter_segment<V, NW>(a, t, s, 1, lds[0], carry);
-  const int end = min(s * a.L + a.L, a.T);
+  const int end = min(s * a.L + a.L, a.T), hi = min(t.hi, end);
   int buf = 0;
   for (int p0 = s * a.L; p0 < end; p0 += NW * kPiece, buf ^= 1) {
     const int q0 = p0 + w * kPiece;
     float u[kPiece][V], x[kPiece][V], h[V];
-    load_piece<T, V>(g, gs, c, cs, q0, t.lo, t.hi, u, x);
+    in.take(q0, t.lo, hi, u, x);
+    const bool full = in.full;
+    in.ask(g, c, q0 + NW * kPiece, t.lo, hi);  // the next round's, behind this one's arithmetic
     if constexpr (NW > 1) {
       float A[V], B[V];
 #pragma unroll
@@ -227,14 +270,14 @@ __global__ __launch_bounds__(NW * 64) void k_recur_fwd(RecurArgs a) {
 #pragma unroll
         for (int i = 0; i < kPiece; ++i) {
           const int p = q0 + i;
-          const bool on = p >= t.lo && p < t.hi;
+          const bool on = full || (p >= t.lo && p < t.hi);
           Pack<T, V> o;
 #pragma unroll
           for (int k = 0; k < V; ++k) {
             h[k] = fmaf(u[i][k], h[k], x[i][k]);
             o.v[k] = st1<T>(on ? h[k] : 0.f);
           }
-          if (p < a.T) stv<T, V>(ho + p * hs, o);
+          if (p < a.T) stv<T, V>(ho.at(p), o);
         }
       }
       if constexpr (NW == 1) {
@@ -259,59 +302,69 @@ __global__ __launch_bounds__(NW * 64) void k_recur_fwd(RecurArgs a) {
 
 // ---- backward ----------------------------------------------------------------------------------
 // SUM: only the segment's (P, Q).
-template <typename T, int V, int NW, bool SUM>
+template <typename T, int V, int NW, bool SUM, bool W>
 __global__ __launch_bounds__(NW * 64) void k_recur_bwd(RecurArgs a) {
   __shared__ float lds[2][NW][64][2 * V];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int s = SUM ? a.S - 1 - (int)blockIdx.y : (int)blockIdx.y;
   const Unit<V> t = unit_of<V>(a, (int64_t)blockIdx.x * 64 + lane);
-  const int sg = a.reverse ? -1 : 1;
-  const T* g = walk((const T*)a.gate, a, a.gr, a.gt, t.r, t.c);
-  const T* c = walk((const T*)a.cand, a, a.cr, a.ct, t.r, t.c);
-  const T* d = a.dh ? walk((const T*)a.dh, a, a.dr, a.dt, t.r, t.c) : nullptr;
-  T* og = walk((T*)a.dgate, a, a.ogr, a.ogt, t.r, t.c);
-  T* oc = walk((T*)a.dcand, a, a.ocr, a.oct, t.r, t.c);
+  const Walk<T, W> g(a.gate, a, a.gr, a.gt, t.r0, t.r, t.c), c(a.cand, a, a.cr, a.ct, t.r0, t.r, t.c);
+  const Walk<T, W> d(a.dh, a, a.dr, a.dt, t.r0, t.r, t.c);
+  const Walk<T, W> og(a.dgate, a, a.ogr, a.ogt, t.r0, t.r, t.c), oc(a.dcand, a, a.ocr, a.oct, t.r0, t.r, t.c);
   float carry[V], span[V];  // carry: gamma, the gradient that reaches the state behind the current stretch
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     carry[k] = !SUM && a.dlast && t.in ? a.dlast[t.ch + k] : 0.f;
     span[k] = 1.f;
   }
-  if constexpr (!SUM && NW > 1)
-    if (a.S > 1) enter_segment<V, NW>(a, t, s, -1, lds[0], carry);
-  const int begin = s * a.L, end = min(begin + a.L, a.T);
-  int buf = 0;
-  for (int p0 = begin + (end - begin - 1) / (NW * kPiece) * (NW * kPiece); p0 >= begin; p0 -= NW * kPiece, buf ^= 1) {
-    const int q0 = p0 + w * kPiece;
-    Pack<T, V> ra[kPiece], rb[kPiece], rd[kPiece];
-    float hp[V];
+  const int begin = s * a.L, end = min(begin + a.L, a.T), lo = max(t.lo, begin);
+  const int top = begin + (end - begin - 1) / (NW * kPiece) * (NW * kPiece);
+  Pack<T, V> ra[kPiece], rb[kPiece], rd[kPiece];
+  Pack<float, V> st;
+  bool asked;  // all of the wave's steps act
+  auto ask = [&](int q0) {
+    asked = __all(q0 >= lo && q0 + kPiece <= t.hi);
+    if (asked) {
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) {
-      const int p = q0 + i;
-      if (p >= t.lo && p < t.hi) {
-        ra[i] = ldv<T, V>(g + sg * p * a.gt);
-        if constexpr (!SUM) rb[i] = ldv<T, V>(c + sg * p * a.ct);
-        if (d) rd[i] = ldv<T, V>(d + sg * p * a.dt);
+      for (int i = 0; i < kPiece; ++i) {
+        ra[i] = ldv<T, V>(g.at(q0 + i));
+        if constexpr (!SUM) rb[i] = ldv<T, V>(c.at(q0 + i));
+        if (a.dh) rd[i] = ldv<T, V>(d.at(q0 + i));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) {
+        const int p = q0 + i;
+        if (p >= lo && p < t.hi) {
+          ra[i] = ldv<T, V>(g.at(p));
+          if constexpr (!SUM) rb[i] = ldv<T, V>(c.at(p));
+          if (a.dh) rd[i] = ldv<T, V>(d.at(p));
+        }
       }
     }
-    if constexpr (!SUM) {
-      Pack<float, V> st;
+    if constexpr (!SUM)
+      if (t.in && q0 >= begin && q0 < a.T) st = ldv<float, V>(a.states + (int64_t)(q0 / kPiece) * a.R * a.H + t.ch);
+  };
+  ask(top + w * kPiece);
+  if constexpr (!SUM && NW > 1)
+    if (a.S > 1) enter_segment<V, NW>(a, t, s, -1, lds[0], carry);
+  int buf = 0;
+  for (int p0 = top; p0 >= begin; p0 -= NW * kPiece, buf ^= 1) {
+    const int q0 = p0 + w * kPiece;
+    float hp[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) st.v[k] = 0.f;
-      if (t.in && q0 < a.T) st = ldv<float, V>(a.states + (int64_t)(q0 / kPiece) * a.R * a.H + t.ch);
-#pragma unroll
-      for (int k = 0; k < V; ++k) hp[k] = st.v[k];
-    }
+    for (int k = 0; k < V; ++k) hp[k] = st.v[k];
     float u[kPiece][V], e[kPiece][V], dgf[kPiece][V], vv[kPiece][V];  // e: dh; dgf: (h_{t-1} - c) u v
+    const bool full = asked;
 #pragma unroll
     for (int i = 0; i < kPiece; ++i) {
-      const bool on = q0 + i >= t.lo && q0 + i < t.hi;
+      const bool on = full || (q0 + i >= t.lo && q0 + i < t.hi);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         float uu, v1;
-        gate_uv(ld1(ra[i].v[k]), uu, v1);
+        gate_uv<T>(ld1(ra[i].v[k]), uu, v1);
         u[i][k] = on ? uu : 1.f;
-        e[i][k] = on && d ? ld1(rd[i].v[k]) : 0.f;
+        e[i][k] = on && a.dh ? ld1(rd[i].v[k]) : 0.f;
         if constexpr (!SUM) {
           const float cc = ld1(rb[i].v[k]);
           dgf[i][k] = on ? (hp[k] - cc) * (uu * v1) : 0.f;
@@ -320,6 +373,7 @@ __global__ __launch_bounds__(NW * 64) void k_recur_bwd(RecurArgs a) {
         }
       }
     }
+    ask(q0 - NW * kPiece);  // the next round's, behind this one's arithmetic
     float gam[V];
     if constexpr (NW > 1) {
       float P[V], Q[V];
@@ -364,14 +418,14 @@ __global__ __launch_bounds__(NW * 64) void k_recur_bwd(RecurArgs a) {
           for (int k = 0; k < V; ++k) {
             const float gg = e[i][k] + gam[k];
             // a step that does not act passes gamma on as it is; its own gradients are zero whatever gamma is
-            const bool on = p >= t.lo && p < t.hi;
+            const bool on = full || (p >= t.lo && p < t.hi);
             pg.v[k] = st1<T>(on ? gg * dgf[i][k] : 0.f);
             pc.v[k] = st1<T>(on ? gg * vv[i][k] : 0.f);
             gam[k] = u[i][k] * gg;
           }
           if (p < a.T) {
-            stv<T, V>(og + sg * p * a.ogt, pg);
-            stv<T, V>(oc + sg * p * a.oct, pc);
+            stv<T, V>(og.at(p), pg);
+            stv<T, V>(oc.at(p), pc);
           }
         }
       }
@@ -410,7 +464,7 @@ __global__ __launch_bounds__(256) void k_recur_step(const T* __restrict__ gate, 
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     float uu, vv;
-    gate_uv(ld1(a.v[k]), uu, vv);
+    gate_uv<T>(ld1(a.v[k]), uu, vv);
     s.v[k] = fmaf(uu, s.v[k], vv * ld1(b.v[k]));
     o.v[k] = st1<T>(s.v[k]);
   }
@@ -419,6 +473,15 @@ __global__ __launch_bounds__(256) void k_recur_step(const T* __restrict__ gate, 
 }
 
 // How the work is cut.  `waves`: waves of 64 lanes that the channels alone give.
+#ifndef DSSM_CW
+#define DSSM_CW 1024
+#endif
+#ifndef DSSM_TGT
+#define DSSM_TGT 4096
+#endif
+#ifndef DSSM_NWM
+#define DSSM_NWM 8
+#endif
 struct Cut {
   int V, NW, S, L;
 };
@@ -430,9 +493,9 @@ Cut cut_of(int64_t R, int T, int H, int dtype) {
   const int pieces = (T + kPiece - 1) / kPiece;
   c.NW = 1;
   c.S = 1;
-  if (waves < 1024 && pieces > 1) {
-    c.NW = pieces >= 5 ? 8 : 4;
-    const int64_t want = 2048 / (waves * c.NW);
+  if (waves < DSSM_CW && pieces > 1) {
+    c.NW = pieces >= DSSM_NWM/2+1 ? DSSM_NWM : 4;
+    const int64_t want = DSSM_TGT / (waves * c.NW);
     if (want >= 2) c.S = (int)std::min<int64_t>(want, (pieces + 2 * c.NW - 1) / (2 * c.NW));
   }
   const int round = c.NW * kPiece, per = (T + c.S - 1) / c.S;
@@ -446,24 +509,24 @@ bool recur_dims_ok(int64_t R, int T, int H) {
          (R * H + 63) / 64 <= 0x7fffffff;
 }
 
-template <typename T, int V, bool FWD>
+template <typename T, int V, bool FWD, bool W>
 void launch(const RecurArgs& a, const Cut& c, hipStream_t s) {
   const dim3 grid((unsigned)((a.R * a.upr + 63) / 64), (unsigned)c.S);
   auto go = [&](auto nw) {
     constexpr int NW = decltype(nw)::value;
     if constexpr (FWD) {
       if constexpr (NW > 1)
-        if (c.S > 1) hipLaunchKernelGGL((k_recur_fwd<T, V, NW, true>), grid, dim3(NW * 64), 0, s, a);
-      hipLaunchKernelGGL((k_recur_fwd<T, V, NW, false>), grid, dim3(NW * 64), 0, s, a);
+        if (c.S > 1) hipLaunchKernelGGL((k_recur_fwd<T, V, NW, true, W>), grid, dim3(NW * 64), 0, s, a);
+      hipLaunchKernelGGL((k_recur_fwd<T, V, NW, false, W>), grid, dim3(NW * 64), 0, s, a);
     } else {
       if constexpr (NW > 1)
-        if (c.S > 1) hipLaunchKernelGGL((k_recur_bwd<T, V, NW, true>), grid, dim3(NW * 64), 0, s, a);
-      hipLaunchKernelGGL((k_recur_bwd<T, V, NW, false>), grid, dim3(NW * 64), 0, s, a);
+        if (c.S > 1) hipLaunchKernelGGL((k_recur_bwd<T, V, NW, true, W>), grid, dim3(NW * 64), 0, s, a);
+      hipLaunchKernelGGL((k_recur_bwd<T, V, NW, false, W>), grid, dim3(NW * 64), 0, s, a);
     }
   };
   if (c.NW == 1) go(std::integral_constant<int, 1>{});
   else if (c.NW == 4) go(std::integral_constant<int, 4>{});
-  else go(std::integral_constant<int, 8>{});
+  else go(std::integral_constant<int, DSSM_NWM>{});
 }
 template <bool FWD>
 int run(RecurArgs& a, int dtype, void* stream) {
@@ -471,13 +534,22 @@ int run(RecurArgs& a, int dtype, void* stream) {
   a.upr = a.H / c.V;
   a.S = c.S;
   a.L = c.L;
+  // a wave's 64 units lie in at most 64 / upr + 2 rows: do all their offsets fit 32 bits?
+  int64_t far = 0;
+  for (int64_t sr : {a.gr, a.cr, a.hr, a.dr, a.ogr, a.ocr}) far = std::max(far, sr < 0 ? INT64_MAX / 256 : sr);
+  const bool wide = (double)far * (64 / a.upr + 2) + a.H >= 1e9;
   by_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
+    auto go = [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      if (wide) launch<T, V, FWD, true>(a, c, (hipStream_t)stream);
+      else launch<T, V, FWD, false>(a, c, (hipStream_t)stream);
+    };
     if constexpr (sizeof(T) == 4) {
-      launch<T, 1, FWD>(a, c, (hipStream_t)stream);
+      go(std::integral_constant<int, 1>{});
     } else {
-      if (c.V == 2) launch<T, 2, FWD>(a, c, (hipStream_t)stream);
-      else launch<T, 1, FWD>(a, c, (hipStream_t)stream);
+      if (c.V == 2) go(std::integral_constant<int, 2>{});
+      else go(std::integral_constant<int, 1>{});
     }
   });
   return seq_status(hipGetLastError());

@@ -28,7 +28,7 @@ from . import _lib
 _CODE = {torch.float32: _lib.DSSM_F32, torch.bfloat16: _lib.DSSM_BF16, torch.float16: _lib.DSSM_F16}
 BLOCK = 128          # columns that share a scale
 MAX_NORM_COLS = 16384
-_PIECE = 16          # include/dssm.h DSSM_RECUR_PIECE
+_PIECE = 8           # include/dssm.h DSSM_RECUR_PIECE
 
 
 class Blocks8(NamedTuple):

@@ -29,9 +29,11 @@ def lookup_grad(dy, ids, V, scale):
     return g * scale, a * abs(scale), torch.bincount(ids, minlength=V).double()[:, None]
 
 
-# One step's own error, relative to the magnitudes it adds: u and v are within 4 units in the last place of
-# fp32 (2^x 1, its correction 1/2, 1 + e 1/2, the reciprocal 1, a product 1/2; a unit is at most 2^-23), the
-# two products and the sum add 3 half units: 4 * 2^-23 + 3 * 2^-24 < 2^-20.  A piece's product of u and the
+# One step's own error, relative to the magnitudes it adds: for fp32 gates u and v are within 4 units in the last
+# place of fp32 (2^x 1, its correction 1/2, 1 + e 1/2, the reciprocal 1, a product 1/2; a unit is at most 2^-23),
+# the two products and the sum add 3 half units: 4 * 2^-23 + 3 * 2^-24 < 2^-20.  For 16-bit gates the correction is
+# left out: 2^x's argument -|f| log2 e is off by half a unit and by log2 e's own 1/4, which moves e, and with
+# it the smaller of u and v (the larger less), by up to |f| * 1.5 * 2^-24.  A piece's product of u and the
 # folds of pieces and segments make the same roundings in another order; twice the bound covers both walks.
 # The roundings are relative to the magnitudes that are added, not to the sum: a piece's map A h + B is formed
 # apart from the h it meets, so where A h and B cancel, the errors of each stay.  Both walks therefore carry the
@@ -39,8 +41,13 @@ def lookup_grad(dy, ids, V, scale):
 STEP = 2.0 ** -19
 
 
+def step_error(gate):
+    return STEP + (0.0 if gate.dtype == torch.float32 else 2 * 1.5 * 2.0 ** -24) * gate.double().abs()
+
+
 def recurrence(gate, cand, lens=None, h0=None, reverse=False):
     """(h, last, states before each step, error bound of h and last)"""
+    step = step_error(gate)
     gate, cand = gate.double(), cand.double()
     R, T, H = gate.shape
     lens = torch.full((R,), T) if lens is None else lens.long().clamp(0, T)
@@ -53,7 +60,7 @@ def recurrence(gate, cand, lens=None, h0=None, reverse=False):
         before[:, t] = s
         x, hu = v[:, t] * cand[:, t], u[:, t] * s
         nm = u[:, t] * m + x.abs()
-        new, ne = hu + x, u[:, t] * e + STEP * nm
+        new, ne = hu + x, u[:, t] * e + step[:, t] * nm
         s, e, m = torch.where(on, new, s), torch.where(on, ne, e), torch.where(on, nm, m)
         h[:, t], err[:, t] = torch.where(on, s, 0.0), torch.where(on, e, 0.0)
     return h, s, before, err, e
@@ -62,6 +69,7 @@ def recurrence(gate, cand, lens=None, h0=None, reverse=False):
 def recurrence_grad(gate, cand, dh, dlast=None, lens=None, h0=None, reverse=False):
     """(dgate, dcand, dh0) and their error bounds"""
     h, _, before, herr, _ = recurrence(gate, cand, lens, h0, reverse)
+    step = step_error(gate)
     gate, cand = gate.double(), cand.double()
     R, T, H = gate.shape
     lens = torch.full((R,), T) if lens is None else lens.long().clamp(0, T)
@@ -78,11 +86,11 @@ def recurrence_grad(gate, cand, dh, dlast=None, lens=None, h0=None, reverse=Fals
         gerr = ge + 2.0 ** -24 * mg
         diff, uv = before[:, t] - cand[:, t], u[:, t] * v[:, t]
         dg, dc = g * diff * uv, g * v[:, t]
-        dge = (gerr * diff.abs() + g.abs() * (emax + 2.0 ** -24 * diff.abs())) * uv + STEP * 2 * dg.abs()
-        dce = gerr * v[:, t] + STEP * dc.abs()
+        dge = (gerr * diff.abs() + g.abs() * (emax + 2.0 ** -24 * diff.abs())) * uv + step[:, t] * 2 * dg.abs()
+        dce = gerr * v[:, t] + step[:, t] * dc.abs()
         for o, val in zip(out, (dg, dc, dge, dce)):
             o[:, t] = torch.where(on, val, 0.0)
-        gam, ge = torch.where(on, u[:, t] * g, gam), torch.where(on, u[:, t] * gerr + STEP * u[:, t] * mg, ge)
+        gam, ge = torch.where(on, u[:, t] * g, gam), torch.where(on, u[:, t] * gerr + step[:, t] * u[:, t] * mg, ge)
         m = torch.where(on, u[:, t] * mg, m)
     return out[0], out[1], gam, out[2], out[3], ge
 
