@@ -29,6 +29,7 @@ namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct Gemm8Args {
   const unsigned char *a, *ea, *w, *ew;
@@ -43,15 +44,17 @@ __device__ __forceinline__ f32x4 mfma8(const i32x8& w, const i32x8& a, f32x4 c, 
 }
 
 // a row's scale bytes of blocks kb .. kb + 3 in one word (bytes behind the row's last block: zero)
+__device__ __forceinline__ unsigned scale_word(const unsigned char* p) {
+  unsigned v;
+  __builtin_memcpy(&v, p, 4);
+  return v;
+}
 __device__ __forceinline__ unsigned scale4(const unsigned char* row, int kb, int KB) {
+  if (kb + 4 <= KB) return scale_word(row + kb);
   unsigned v = 0;
-  if (kb + 4 <= KB) {
-    __builtin_memcpy(&v, row + kb, 4);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (kb + i < KB) v |= (unsigned)row[kb + i] << (8 * i);
-  }
+  for (int i = 0; i < 3; ++i)
+    if (kb + i < KB) v |= (unsigned)row[kb + i] << (8 * i);
   return v;
 }
 
@@ -66,17 +69,30 @@ __device__ __forceinline__ void store4(const Gemm8Args& g, int m, int n, f32x4 v
 }
 
 // ---- tiles -------------------------------------------------------------------------------------
-// A workgroup of WM x WN waves computes (WM MI 16) x (WN NI 16) outputs.  Both operands' blocks of 128
-// columns go from memory straight to LDS, 16 bytes a lane, into one half of a double buffer while the
-// other is multiplied.  A row's 128 bytes are eight 16-byte pieces; piece p of row r lies at p ^ (r & 7),
-// so that the 16 rows a fragment read touches spread over all banks.  The direct load writes LDS in lane
-// order, so the permutation is applied to the address each lane loads from.
+// A workgroup of WM x WN waves computes (WM MI 32) x (WN NI 32) outputs with v_mfma_scale_f32_32x32x64.
+//
+// Both operands go from memory straight to LDS, 16 bytes a lane, a block of 128 columns at a time into one half of
+// a double buffer; whole 128-byte lines, because the two halves of a line that are asked for apart meet as
+// one pending line in the vector cache and stall it.  A block is multiplied in two rounds of 64 columns, and a
+// round multiplies fragments that are in registers already while it reads the next round's: when a block's
+// second round begins, nobody needs its LDS half any more, and the block after the next is asked for, two
+// rounds of products (2048 cycles of the matrix units) before its first fragment is read.
+//
+// A row's 128 bytes are eight 16-byte pieces; piece p of row r lies at p ^ (r >> 1 & 7).  A 16-byte read serves
+// sixteen lanes a cycle: lanes 0-3, 12-15, 20-23 and 24-27 of a half wave, then the others (found with the
+// conflict counter, which reads zero); of these rows no two of the same parity have the same r >> 1 & 7, so
+// they cover all 64 banks.  The direct load writes LDS in lane order, so the permutation is applied to the
+// address that each lane loads from.
 template <int WM, int WN, int MI, int NI, typename O>
-__global__ __launch_bounds__(WM * WN * 64) void k_gemm8(Gemm8Args g) {
-  constexpr int BM = WM * MI * 16, BN = WN * NI * 16, NW = WM * WN, kLoads = (BM + BN) / 8 / NW;
-  static_assert((BM + BN) / 8 % NW == 0 && BM / 8 % NW == 0, "every wave loads the same number of 8-row stripes");
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2][(BM + BN) * kBlk];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, wm = wv % WM, wn = wv / WM;
+__global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Gemm8Args g) {
+  constexpr int BM = WM * MI * 32, BN = WN * NI * 32, NW = WM * WN, kLoads = (BM + BN) / 8 / NW;
+  static_assert(kLoads * 8 * NW == BM + BN && BM % 8 == 0, "every wave loads the same number of 8-row stripes");
+  static_assert(BM + BN == NW * 64 && BM % 64 == 0, "a row's scales are loaded by one thread");
+  // two blocks, then two words of scales a row.  One object: of two the compiler knows that they are two, tells
+  // the direct loads apart by that, and puts a wait for all of them in front of every read.
+  constexpr int kBuf = (BM + BN) * kBlk;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kBuf + 2 * (BM + BN) * 4];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % WM, wn = wv / WM;
   const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN;
   // neighbouring tiles to one XCD, in bands of 8 tile rows whose operands its L2 keeps
   int t = xcd_tile(blockIdx.x, tm * tn);
@@ -84,82 +100,150 @@ __global__ __launch_bounds__(WM * WN * 64) void k_gemm8(Gemm8Args g) {
   const int band = t / (kBand * tn), rows = min(kBand, tm - band * kBand);
   t -= band * kBand * tn;
   const int m0 = (band * kBand + t % rows) * BM, n0 = t / rows * BN;
-  const int64_t Kp = (int64_t)g.KB * kBlk;
+  const unsigned Kp = (unsigned)g.KB * kBlk;  // (a tile's rows span less than 2^32 bytes: checked on the host)
 
-  // stripe i of this wave: rows 8 (wv + i NW) ... of the tile's BM + BN rows, a's first
-  const unsigned char* src[kLoads];
+  // stripe i of this wave: rows 8 (wv + i NW) ... of the tile's BM + BN rows, a's first; rows behind the last
+  // one read the last one (their outputs are not stored)
+  const unsigned char* base[kLoads];
+  unsigned off[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    const int r = (wv + i * NW) * 8 + (lane >> 3), p = (lane & 7) ^ (r & 7);
-    const bool isa = r < BM;
-    const int row = isa ? min(m0 + r, g.M - 1) : min(n0 + r - BM, g.N - 1);
-    src[i] = (isa ? g.a : g.w) + (int64_t)row * Kp + p * 16;
+    const int r0 = (wv + i * NW) * 8, r = r0 + (lane >> 3), p = (lane & 7) ^ (r >> 1 & 7);
+    const bool isa = r0 < BM;
+    base[i] = isa ? g.a + (int64_t)m0 * Kp : g.w + (int64_t)n0 * Kp;
+    off[i] = (unsigned)(isa ? min(r, g.M - 1 - m0) : min(r - BM, g.N - 1 - n0)) * Kp + p * 16;
   }
-  auto load = [&](int kb, int buf) {
+  // (behind the last block the last one is loaded again, into a half that serves no more: no branch)
+  auto load = [&](int kb) {
+    const unsigned at = (unsigned)min(kb, g.KB - 1) * kBlk;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(src[i] + (int64_t)kb * kBlk),
-                                       (__attribute__((address_space(3))) unsigned*)&lds[buf][(wv + i * NW) * 1024], 16, 0,
-                                       0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(base[i] + at + off[i]),
+                                       (__attribute__((address_space(3))) unsigned*)&lds[(kb & 1) * kBuf + (wv + i * NW) * 1024],
+                                       16, 0, 0);
   };
-  const unsigned char* ea[MI];
-  const unsigned char* ew[NI];
-#pragma unroll
-  for (int i = 0; i < MI; ++i) ea[i] = g.ea + (int64_t)min(m0 + (wm * MI + i) * 16 + (lane & 15), g.M - 1) * g.KB;
-#pragma unroll
-  for (int j = 0; j < NI; ++j) ew[j] = g.ew + (int64_t)min(n0 + (wn * NI + j) * 16 + (lane & 15), g.N - 1) * g.KB;
-  unsigned sa[MI], sw[NI];
+  // Scales: thread t holds row t's of four blocks in one word, asked for three blocks ahead and written to LDS
+  // two ahead.  (The last word of a row starts at KB - 4 and is shifted down.)
+  const int st = threadIdx.x;
+  const unsigned char* srow = st < BM ? g.ea + (int64_t)min(m0 + st, g.M - 1) * g.KB : g.ew + (int64_t)min(n0 + st - BM, g.N - 1) * g.KB;
+  unsigned sword;
+  auto ask_scales = [&](int kb) { sword = scale_word(srow + min(kb, g.KB - 4)); };
+  auto put_scales = [&](int kb) {
+    const int behind = g.KB >= 4 ? max(0, kb + 4 - g.KB) : 0;
+    *reinterpret_cast<unsigned*>(&lds[2 * kBuf + ((kb >> 2 & 1) * (BM + BN) + st) * 4]) = sword >> (8 * behind);
+  };
+  const int fr = lane & 31, fg = lane >> 5;
 
-  f32x4 acc[MI][NI];
+  f32x16 acc[MI][NI];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NI; ++j) acc[i][j] = f32x16{};
 
-  // a fragment: lane l holds 32 of row l % 16's bytes, the pieces l / 16 and l / 16 + 4 (the order of k
-  // inside a block is free as long as both operands use the same)
-  const int fr = lane & 15, fp = lane >> 4;
-  auto frag = [&](const unsigned char* base, int r) {
-    const i32x4 lo = *reinterpret_cast<const i32x4*>(base + (r + fr) * kBlk + ((fp ^ (fr & 7)) * 16));
-    const i32x4 hi = *reinterpret_cast<const i32x4*>(base + (r + fr) * kBlk + (((fp + 4) ^ (fr & 7)) * 16));
+  // a fragment of half h of a block: lane l holds 32 of row l % 32's bytes, pieces 4 h + 2 (l / 32) and the next (the
+  // order of k inside a block is free as long as both operands use the same)
+  const int sw0 = fr >> 1 & 7, o0 = ((2 * fg) ^ sw0) * 16, o1 = ((2 * fg + 1) ^ sw0) * 16;
+  const int ra = (wm * MI * 32 + fr) * kBlk, rw = (BM + wn * NI * 32 + fr) * kBlk;
+  auto frag = [&](int kb, int h, int row) {
+    const unsigned char* at = lds + (kb & 1) * kBuf + row;
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(at + (o0 ^ h * 64)), hi = *reinterpret_cast<const i32x4*>(at + (o1 ^ h * 64));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-
-  load(0, 0);
-  for (int kb = 0; kb < g.KB; ++kb) {
-    const int buf = kb & 1;
-    if ((kb & 3) == 0) {
+  i32x8 fa[MI], w0[NI], w1[NI];
+  int sa[MI], sw[NI], na[MI], nw[NI];
+  auto fetch_scales = [&](int kb) {
+    const unsigned char* at = lds + 2 * kBuf + (kb >> 2 & 1) * (BM + BN) * 4 + (kb & 3);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) sa[i] = scale4(ea[i], kb, g.KB);
+    for (int i = 0; i < MI; ++i) na[i] = at[((wm * MI + i) * 32 + fr) * 4];
 #pragma unroll
-      for (int j = 0; j < NI; ++j) sw[j] = scale4(ew[j], kb, g.KB);
-    }
-    // this wave's direct loads have landed; behind the barrier all waves' have, and all have finished
-    // reading the half that is loaded next
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (kb + 1 < g.KB) load(kb + 1, buf ^ 1);
-    const unsigned char* A = lds[buf];
-    const unsigned char* W = lds[buf] + BM * kBlk;
-    i32x8 fw[NI];
-#pragma unroll
-    for (int j = 0; j < NI; ++j) fw[j] = frag(W, (wn * NI + j) * 16);
+    for (int j = 0; j < NI; ++j) nw[j] = at[(BM + (wn * NI + j) * 32 + fr) * 4];
+  };
+  // The products of one round on the fragments fa and w; each one, when it has served, is followed by its place
+  // in half h of block kb under the products that follow.  The order is kept by hand: left alone, the
+  // compiler moves each read down to its use.  (The last round reads fragments that nobody multiplies.)
+  auto products = [&](const i32x8 (&w)[NI], i32x8 (&next)[NI], int kb, int h) {
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const i32x8 fa = frag(A, (wm * MI + i) * 16);
 #pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] = mfma8(fw[j], fa, acc[i][j], (int)sw[j], (int)sa[i]);
+      for (int j = 0; j < NI; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[j], fa[i], acc[i][j], 0, 0, 0, sw[j], 0, sa[i]);
+      __builtin_amdgcn_sched_barrier(0);
+      fa[i] = frag(kb, h, ra + i * 32 * kBlk);
+      if (i == 0) {
+#pragma unroll
+        for (int j = 0; j < NI; ++j) next[j] = frag(kb, h, rw + j * 32 * kBlk);
+      }
+      if (i == MI - 2 && h == 0) fetch_scales(kb);
+      __builtin_amdgcn_sched_barrier(0);
     }
+  };
+
+  load(0);
+  sword = scale4(srow, 0, g.KB);
+  put_scales(0);
+  load(1);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < MI; ++i) sa[i] >>= 8;
+  for (int j = 0; j < NI; ++j) w0[j] = frag(0, 0, rw + j * 32 * kBlk);
 #pragma unroll
-    for (int j = 0; j < NI; ++j) sw[j] >>= 8;
+  for (int i = 0; i < MI; ++i) fa[i] = frag(0, 0, ra + i * 32 * kBlk);
+  fetch_scales(0);
+  for (int kb = 0; kb < g.KB; ++kb) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) sa[i] = na[i];
+#pragma unroll
+    for (int j = 0; j < NI; ++j) sw[j] = nw[j];
+    // first half; the second's fragments are in the same LDS half
+    products(w0, w1, kb, 1);
+    // this wave's loads have landed (block kb + 1's are the youngest) and its reads of block kb are done; behind
+    // the barrier all waves' have
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if ((kb & 3) == 2 && kb + 2 < g.KB) put_scales(kb + 2);
+    if ((kb & 3) == 1 && kb + 3 < g.KB) ask_scales(kb + 3);
+    load(kb + 2);
+    products(w1, w0, kb + 1, 0);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may reach LDS that is another workgroup's by then
+  // A lane holds, for output column l % 32 of the instruction (m), rows 8 q + 4 (l / 32) + 0 .. 3 (n): eight bytes of
+  // a row of the result.  The tile is put together in LDS, so that its rows leave in whole lines: stored from
+  // the registers they cost the L2 twelve times the requests.  Piece c (16 bytes) of row r lies at c ^ (r % kPieces).
+  asm volatile("s_barrier" ::: "memory");  // all waves are past their last reads of the operands
+  constexpr int kPieces = BN / 8;
+  static_assert(BM * BN * 2 <= 2 * kBuf && (kPieces & (kPieces - 1)) == 0, "the tile fits where the operands were");
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+  for (int j = 0; j < NI; ++j)
 #pragma unroll
-    for (int j = 0; j < NI; ++j)
-      store4<O>(g, m0 + (wm * MI + i) * 16 + fr, n0 + (wn * NI + j) * 16 + fp * 4, acc[i][j]);
+    for (int q = 0; q < 4; ++q) {
+      const int n = (wn * NI + j) * 32 + 8 * q + 4 * fg;
+      float add[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) add[e] = g.bias && n0 + n + e < g.N ? g.bias[n0 + n + e] : 0.f;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int r = (wm * MI + i) * 32 + fr;
+        Pack<O, 4> y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y.v[e] = st1<O>(acc[i][j][4 * q + e] + add[e]);
+        *reinterpret_cast<uint2*>(&lds[r * BN * 2 + (((n >> 3) ^ (r & (kPieces - 1))) << 4) + (n & 4) * 2]) =
+            __builtin_bit_cast(uint2, y);
+      }
+    }
+  __syncthreads();
+  for (int u = threadIdx.x; u < BM * kPieces; u += NW * 64) {
+    const int r = u / kPieces, c = u % kPieces, n = n0 + c * 8;
+    if (m0 + r >= g.M || n >= g.N) continue;
+    const uint4 y = *reinterpret_cast<const uint4*>(&lds[r * BN * 2 + ((c ^ (r & (kPieces - 1))) << 4)]);
+    const Pack<O, 8> p = __builtin_bit_cast(Pack<O, 8>, y);
+    O* to = (O*)g.out + (int64_t)(m0 + r) * g.ldo + n;
+    if (n + 8 <= g.N) {
+      stv<O, 8>(to, p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n + e < g.N) to[e] = p.v[e];
+    }
+  }
 }
 
 // ---- few rows ----------------------------------------------------------------------------------
@@ -231,9 +315,9 @@ void run_gemm8(const Gemm8Args& g, hipStream_t s) {
   } else if (g.M <= 64 || tiles(128, 128) < 64) {
     hipLaunchKernelGGL((k_gemm8_rows<4, O>), dim3((g.N + 15) / 16, (g.M + 63) / 64), dim3(512), 0, s, g);
   } else if (tiles(256, 256) < 128) {
-    hipLaunchKernelGGL((k_gemm8<2, 2, 4, 4, O>), dim3((unsigned)tiles(128, 128)), dim3(256), 0, s, g);
+    hipLaunchKernelGGL((k_gemm8<2, 2, 2, 2, O>), dim3((unsigned)tiles(128, 128)), dim3(256), 0, s, g);
   } else {
-    hipLaunchKernelGGL((k_gemm8<2, 4, 8, 4, O>), dim3((unsigned)tiles(256, 256)), dim3(512), 0, s, g);
+    hipLaunchKernelGGL((k_gemm8<2, 4, 4, 2, O>), dim3((unsigned)tiles(256, 256)), dim3(512), 0, s, g);
   }
 }
 
@@ -245,7 +329,7 @@ using namespace dssm::seq;
 
 extern "C" int dssm_blocks8_matmul(const void* a, const void* ascale, const void* w, const void* wscale, int64_t M, int64_t N,
                                    int64_t K, const float* bias, void* out, int64_t ldo, int out_dtype, void* stream) {
-  if (M < 0 || N < 0 || K <= 0 || M > (1 << 28) || N > (1 << 24) || K > (1 << 28) || ldo < N || (out_dtype != DSSM_BF16 && out_dtype != DSSM_F16) ||
+  if (M < 0 || N < 0 || K <= 0 || M > (1 << 28) || N > (1 << 24) || K > (1 << 22) || ldo < N || (out_dtype != DSSM_BF16 && out_dtype != DSSM_F16) ||
       (M > 0 && N > 0 && (!a || !ascale || !w || !wscale || !out)) || (uintptr_t)a % 16 || (uintptr_t)w % 16)
     return dssm::report_error(DSSM_E_INVALID, "blocks8_matmul: bad argument (16-byte aligned values, bf16 or fp16 result)");
   if (M == 0 || N == 0) return DSSM_OK;

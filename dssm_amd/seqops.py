@@ -405,8 +405,8 @@ def blocks8_matmul(a: Blocks8, w: Blocks8, bias: Optional[torch.Tensor] = None,
     M, N = _check8(a, "a"), _check8(w, "w")
     if a.cols != w.cols:
         raise ValueError(f"a has {a.cols} columns, w {w.cols}")
-    if M > 1 << 28 or N > 1 << 24 or a.cols > 1 << 28:
-        raise ValueError("at most 2^28 rows, 2^24 outputs and 2^28 columns")
+    if M > 1 << 28 or N > 1 << 24 or a.cols > 1 << 22:
+        raise ValueError("at most 2^28 rows, 2^24 outputs and 2^22 columns")
     bias = _vector(bias, N, "bias")
     dev = _on_gpu(a.q, a.scale, w.q, w.scale, bias)
     out = torch.empty(M, N, dtype=dtype, device=dev)
