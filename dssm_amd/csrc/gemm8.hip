@@ -114,10 +114,10 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
     off[i] = (unsigned)(isa ? min(r, g.M - 1 - m0) : min(r - BM, g.N - 1 - n0)) * Kp + p * 16;
   }
   // (behind the last block the last one is loaded again, into a half that serves no more: no branch)
-  auto load = [&](int kb) {
+  auto load = [&](int kb, int from, int to) {
     const unsigned at = (unsigned)min(kb, g.KB - 1) * kBlk;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
+    for (int i = from; i < to; ++i)
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(base[i] + at + off[i]),
                                        (__attribute__((address_space(3))) unsigned*)&lds[(kb & 1) * kBuf + (wv + i * NW) * 1024],
                                        16, 0, 0);
@@ -159,9 +159,11 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
     for (int j = 0; j < NI; ++j) nw[j] = at[(BM + (wn * NI + j) * 32 + fr) * 4];
   };
   // The products of one round on the fragments fa and w; each one, when it has served, is followed by its place
-  // in half h of block kb under the products that follow.  The order is kept by hand: left alone, the
-  // compiler moves each read down to its use.  (The last round reads fragments that nobody multiplies.)
-  auto products = [&](const i32x8 (&w)[NI], i32x8 (&next)[NI], int kb, int h) {
+  // in half h of block kb under the products that follow.  A second round (h = 0: the next block's first
+  // fragments) also asks for block kb + 1, a part behind each pair of products: asked for at once the loads
+  // fill the vector memory's queue, and the products wait behind them.  The order is kept by hand: left alone,
+  // the compiler moves each read down to its use.  (The last round reads fragments that nobody multiplies.)
+  auto products = [&](const i32x8 (&w)[NI], i32x8 (&next)[NI], int kb, int h, auto&& meet) {
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -169,6 +171,8 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
       for (int j = 0; j < NI; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[j], fa[i], acc[i][j], 0, 0, 0, sw[j], 0, sa[i]);
       __builtin_amdgcn_sched_barrier(0);
+      if (i == 0) meet();
+      if (h == 0) load(kb + 1, i * kLoads / MI, (i + 1) * kLoads / MI);
       fa[i] = frag(kb, h, ra + i * 32 * kBlk);
       if (i == 0) {
 #pragma unroll
@@ -179,10 +183,10 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
     }
   };
 
-  load(0);
+  load(0, 0, kLoads);
   sword = scale4(srow, 0, g.KB);
   put_scales(0);
-  load(1);
+  load(1, 0, kLoads);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
   for (int j = 0; j < NI; ++j) w0[j] = frag(0, 0, rw + j * 32 * kBlk);
@@ -195,14 +199,14 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
 #pragma unroll
     for (int j = 0; j < NI; ++j) sw[j] = nw[j];
     // first half; the second's fragments are in the same LDS half
-    products(w0, w1, kb, 1);
-    // this wave's loads have landed (block kb + 1's are the youngest) and its reads of block kb are done; behind
-    // the barrier all waves' have
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if ((kb & 3) == 2 && kb + 2 < g.KB) put_scales(kb + 2);
-    if ((kb & 3) == 1 && kb + 3 < g.KB) ask_scales(kb + 3);
-    load(kb + 2);
-    products(w1, w0, kb + 1, 0);
+    products(w0, w1, kb, 1, [] {});
+    // second half, and under its first products: this wave's loads have landed (block kb + 1's are the youngest)
+    // and its reads of block kb are done; behind the barrier all waves' have
+    products(w1, w0, kb + 1, 0, [&] {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if ((kb & 3) == 2 && kb + 2 < g.KB) put_scales(kb + 2);
+      if ((kb & 3) == 1 && kb + 3 < g.KB) ask_scales(kb + 3);
+    });
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may reach LDS that is another workgroup's by then
   // A lane holds, for output column l % 32 of the instruction (m), rows 8 q + 4 (l / 32) + 0 .. 3 (n): eight bytes of
