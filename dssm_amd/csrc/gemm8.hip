@@ -87,7 +87,8 @@ template <int WM, int WN, int MI, int NI, typename O>
 __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Gemm8Args g) {
   constexpr int BM = WM * MI * 32, BN = WN * NI * 32, NW = WM * WN, kLoads = (BM + BN) / 8 / NW;
   static_assert(kLoads * 8 * NW == BM + BN && BM % 8 == 0, "every wave loads the same number of 8-row stripes");
-  static_assert(BM + BN == NW * 64 && BM % 64 == 0, "a row's scales are loaded by one thread");
+  constexpr int kScaleRows = (BM + BN) / (NW * 64);  // a thread's
+  static_assert(kScaleRows * NW * 64 == BM + BN && BM % 64 == 0, "a row's scales are loaded by one thread");
   // two blocks, then two words of scales a row.  One object: of two the compiler knows that they are two, tells
   // the direct loads apart by that, and puts a wait for all of them in front of every read.
   constexpr int kBuf = (BM + BN) * kBlk;
@@ -122,15 +123,26 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
                                        (__attribute__((address_space(3))) unsigned*)&lds[(kb & 1) * kBuf + (wv + i * NW) * 1024],
                                        16, 0, 0);
   };
-  // Scales: thread t holds row t's of four blocks in one word, asked for three blocks ahead and written to LDS
+  // Scales: a thread holds a row's of four blocks in one word, asked for three blocks ahead and written to LDS
   // two ahead.  (The last word of a row starts at KB - 4 and is shifted down.)
-  const int st = threadIdx.x;
-  const unsigned char* srow = st < BM ? g.ea + (int64_t)min(m0 + st, g.M - 1) * g.KB : g.ew + (int64_t)min(n0 + st - BM, g.N - 1) * g.KB;
-  unsigned sword;
-  auto ask_scales = [&](int kb) { sword = scale_word(srow + min(kb, g.KB - 4)); };
+  const unsigned char* srow[kScaleRows];
+  unsigned sword[kScaleRows];
+#pragma unroll
+  for (int i = 0; i < kScaleRows; ++i) {
+    const int r = i * NW * 64 + threadIdx.x;
+    srow[i] = r < BM ? g.ea + (int64_t)min(m0 + r, g.M - 1) * g.KB : g.ew + (int64_t)min(n0 + r - BM, g.N - 1) * g.KB;
+    sword[i] = scale4(srow[i], 0, g.KB);
+  }
+  auto ask_scales = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < kScaleRows; ++i) sword[i] = scale_word(srow[i] + min(kb, g.KB - 4));
+  };
   auto put_scales = [&](int kb) {
     const int behind = g.KB >= 4 ? max(0, kb + 4 - g.KB) : 0;
-    *reinterpret_cast<unsigned*>(&lds[2 * kBuf + ((kb >> 2 & 1) * (BM + BN) + st) * 4]) = sword >> (8 * behind);
+#pragma unroll
+    for (int i = 0; i < kScaleRows; ++i)
+      *reinterpret_cast<unsigned*>(&lds[2 * kBuf + ((kb >> 2 & 1) * (BM + BN) + i * NW * 64 + threadIdx.x) * 4]) =
+          sword[i] >> (8 * behind);
   };
   const int fr = lane & 31, fg = lane >> 5;
 
@@ -184,7 +196,6 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
   };
 
   load(0, 0, kLoads);
-  sword = scale4(srow, 0, g.KB);
   put_scales(0);
   load(1, 0, kLoads);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
