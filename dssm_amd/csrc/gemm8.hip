@@ -71,28 +71,34 @@ __device__ __forceinline__ void store4(const Gemm8Args& g, int m, int n, f32x4 v
 // ---- tiles -------------------------------------------------------------------------------------
 // A workgroup of WM x WN waves computes (WM MI 32) x (WN NI 32) outputs with v_mfma_scale_f32_32x32x64.
 //
-// Both operands go from memory straight to LDS, 16 bytes a lane, a block of 128 columns at a time into one half of
-// a double buffer; whole 128-byte lines, because the two halves of a line that are asked for apart meet as
-// one pending line in the vector cache and stall it.  A block is multiplied in two rounds of 64 columns, and a
-// round multiplies fragments that are in registers already while it reads the next round's: when a block's
-// second round begins, nobody needs its LDS half any more, and the block after the next is asked for, two
-// rounds of products (2048 cycles of the matrix units) before its first fragment is read.
+// Both operands go from memory straight to LDS, 16 bytes a lane, a block of 128 columns at a time into one of D
+// buffers; whole 128-byte lines, because the two halves of a line that are asked for apart meet as one pending
+// line in the vector cache and stall it.  A block is multiplied in two rounds of 64 columns, and a round
+// multiplies fragments that are in registers already while it reads the next round's: when a block's second
+// round begins, nobody needs its buffer any more, and the block D further on is asked for, 2 (D - 1) rounds of
+// products before its first fragment is read.  D is 2 for the large tiles (256 x 256: 128 KB of LDS, 2048 cycles
+// of the matrix units ahead); 64 x 64, which runs where there are few tiles and the memory's latency is all
+// there is to a block, takes 4.
 //
 // A row's 128 bytes are eight 16-byte pieces; piece p of row r lies at p ^ (r >> 1 & 7).  A 16-byte read serves
 // sixteen lanes a cycle: lanes 0-3, 12-15, 20-23 and 24-27 of a half wave, then the others (found with the
 // conflict counter, which reads zero); of these rows no two of the same parity have the same r >> 1 & 7, so
 // they cover all 64 banks.  The direct load writes LDS in lane order, so the permutation is applied to the
 // address that each lane loads from.
-template <int WM, int WN, int MI, int NI, typename O>
+template <int WM, int WN, int MI, int NI, int D, typename O>
 __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Gemm8Args g) {
   constexpr int BM = WM * MI * 32, BN = WN * NI * 32, NW = WM * WN, kLoads = (BM + BN) / 8 / NW;
   static_assert(kLoads * 8 * NW == BM + BN && BM % 8 == 0, "every wave loads the same number of 8-row stripes");
-  constexpr int kScaleRows = (BM + BN) / (NW * 64);  // a thread's
-  static_assert(kScaleRows * NW * 64 == BM + BN && BM % 64 == 0, "a row's scales are loaded by one thread");
-  // two blocks, then two words of scales a row.  One object: of two the compiler knows that they are two, tells
-  // the direct loads apart by that, and puts a wait for all of them in front of every read.
-  constexpr int kBuf = (BM + BN) * kBlk;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kBuf + 2 * (BM + BN) * 4];
+  // Scales.  The large tiles keep a word a row, four blocks' bytes, which a thread loads for a row at a time.  The
+  // small one sends a byte a row and block the operands' way (the load widens it to a word): no wait of its own,
+  // for more work in the vector cache, which they leave idle.
+  constexpr bool kWords = D == 2;
+  constexpr int kScaleRows = (BM + BN) / (NW * 64) ? (BM + BN) / (NW * 64) : 1;  // a thread's
+  static_assert(BM % 64 == 0 && (kScaleRows * NW * 64 == BM + BN || !kWords), "a row's scales are loaded by one thread");
+  // D blocks, then the scales.  One object: of two the compiler knows that they are two, tells the direct loads
+  // apart by that, and puts a wait for all of them in front of every read.
+  constexpr int kBuf = (BM + BN) * kBlk, kScale = (BM + BN) * 4;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[D * kBuf + D * kScale];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % WM, wn = wv / WM;
   const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN;
   // neighbouring tiles to one XCD, in bands of 8 tile rows whose operands its L2 keeps
@@ -120,18 +126,18 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
 #pragma unroll
     for (int i = from; i < to; ++i)
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(base[i] + at + off[i]),
-                                       (__attribute__((address_space(3))) unsigned*)&lds[(kb & 1) * kBuf + (wv + i * NW) * 1024],
+                                       (__attribute__((address_space(3))) unsigned*)&lds[(kb & (D - 1)) * kBuf + (wv + i * NW) * 1024],
                                        16, 0, 0);
   };
-  // Scales: a thread holds a row's of four blocks in one word, asked for three blocks ahead and written to LDS
-  // two ahead.  (The last word of a row starts at KB - 4 and is shifted down.)
+  // Words: asked for three blocks ahead and written to LDS two ahead (the last word of a row starts at KB - 4 and
+  // is shifted down).  Bytes: the waves that have a row load block kb + D's with its operands.
   const unsigned char* srow[kScaleRows];
   unsigned sword[kScaleRows];
 #pragma unroll
   for (int i = 0; i < kScaleRows; ++i) {
     const int r = i * NW * 64 + threadIdx.x;
     srow[i] = r < BM ? g.ea + (int64_t)min(m0 + r, g.M - 1) * g.KB : g.ew + (int64_t)min(n0 + r - BM, g.N - 1) * g.KB;
-    sword[i] = scale4(srow[i], 0, g.KB);
+    if (kWords) sword[i] = scale4(srow[i], 0, g.KB);
   }
   auto ask_scales = [&](int kb) {
 #pragma unroll
@@ -141,8 +147,17 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
     const int behind = g.KB >= 4 ? max(0, kb + 4 - g.KB) : 0;
 #pragma unroll
     for (int i = 0; i < kScaleRows; ++i)
-      *reinterpret_cast<unsigned*>(&lds[2 * kBuf + ((kb >> 2 & 1) * (BM + BN) + i * NW * 64 + threadIdx.x) * 4]) =
+      *reinterpret_cast<unsigned*>(&lds[D * kBuf + (kb >> 2 & 1) * kScale + (i * NW * 64 + threadIdx.x) * 4]) =
           sword[i] >> (8 * behind);
+  };
+  auto load_scales = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < kScaleRows; ++i)
+      if ((i * NW + wv) * 64 < BM + BN)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(srow[i] + min(kb, g.KB - 1)),
+                                         (__attribute__((address_space(3))) unsigned*)&lds[D * kBuf + (kb & (D - 1)) * kScale +
+                                                                                            (i * NW + wv) * 256],
+                                         1, 0, 0);
   };
   const int fr = lane & 31, fg = lane >> 5;
 
@@ -157,14 +172,14 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
   const int sw0 = fr >> 1 & 7, o0 = ((2 * fg) ^ sw0) * 16, o1 = ((2 * fg + 1) ^ sw0) * 16;
   const int ra = (wm * MI * 32 + fr) * kBlk, rw = (BM + wn * NI * 32 + fr) * kBlk;
   auto frag = [&](int kb, int h, int row) {
-    const unsigned char* at = lds + (kb & 1) * kBuf + row;
+    const unsigned char* at = lds + (kb & (D - 1)) * kBuf + row;
     const i32x4 lo = *reinterpret_cast<const i32x4*>(at + (o0 ^ h * 64)), hi = *reinterpret_cast<const i32x4*>(at + (o1 ^ h * 64));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
   i32x8 fa[MI], w0[NI], w1[NI];
   int sa[MI], sw[NI], na[MI], nw[NI];
   auto fetch_scales = [&](int kb) {
-    const unsigned char* at = lds + 2 * kBuf + (kb >> 2 & 1) * (BM + BN) * 4 + (kb & 3);
+    const unsigned char* at = lds + D * kBuf + (kWords ? (kb >> 2 & 1) * kScale + (kb & 3) : (kb & (D - 1)) * kScale);
 #pragma unroll
     for (int i = 0; i < MI; ++i) na[i] = at[((wm * MI + i) * 32 + fr) * 4];
 #pragma unroll
@@ -172,7 +187,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
   };
   // The products of one round on the fragments fa and w; each one, when it has served, is followed by its place
   // in half h of block kb under the products that follow.  A second round (h = 0: the next block's first
-  // fragments) also asks for block kb + 1, a part behind each pair of products: asked for at once the loads
+  // fragments) also asks for block kb + D - 1, a part behind each pair of products: asked for at once the loads
   // fill the vector memory's queue, and the products wait behind them.  The order is kept by hand: left alone,
   // the compiler moves each read down to its use.  (The last round reads fragments that nobody multiplies.)
   auto products = [&](const i32x8 (&w)[NI], i32x8 (&next)[NI], int kb, int h, auto&& meet) {
@@ -184,20 +199,23 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[j], fa[i], acc[i][j], 0, 0, 0, sw[j], 0, sa[i]);
       __builtin_amdgcn_sched_barrier(0);
       if (i == 0) meet();
-      if (h == 0) load(kb + 1, i * kLoads / MI, (i + 1) * kLoads / MI);
+      if (h == 0) load(kb + D - 1, i * kLoads / MI, (i + 1) * kLoads / MI);
       fa[i] = frag(kb, h, ra + i * 32 * kBlk);
       if (i == 0) {
 #pragma unroll
         for (int j = 0; j < NI; ++j) next[j] = frag(kb, h, rw + j * 32 * kBlk);
       }
-      if (i == MI - 2 && h == 0) fetch_scales(kb);
+      if (i == (MI > 1 ? MI - 2 : 0) && h == 0) fetch_scales(kb);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  load(0, 0, kLoads);
-  put_scales(0);
-  load(1, 0, kLoads);
+#pragma unroll
+  for (int kb = 0; kb < D; ++kb) {
+    load(kb, 0, kLoads);
+    if (!kWords) load_scales(kb);
+  }
+  if (kWords) put_scales(0);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
   for (int j = 0; j < NI; ++j) w0[j] = frag(0, 0, rw + j * 32 * kBlk);
@@ -211,12 +229,19 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
     for (int j = 0; j < NI; ++j) sw[j] = nw[j];
     // first half; the second's fragments are in the same LDS half
     products(w0, w1, kb, 1, [] {});
-    // second half, and under its first products: this wave's loads have landed (block kb + 1's are the youngest)
-    // and its reads of block kb are done; behind the barrier all waves' have
+    // second half, and under its first products: this wave's loads of block kb + 1 have landed (all but the D - 2
+    // younger blocks'; a wave without scale rows of its own has no more than kLoads of them a block) and its reads
+    // of block kb are done; behind the barrier all waves' have
     products(w1, w0, kb + 1, 0, [&] {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if ((kb & 3) == 2 && kb + 2 < g.KB) put_scales(kb + 2);
-      if ((kb & 3) == 1 && kb + 3 < g.KB) ask_scales(kb + 3);
+      if constexpr (kWords) {
+        static_assert(D == 2, "nothing younger is in flight");
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if ((kb & 3) == 2 && kb + 2 < g.KB) put_scales(kb + 2);
+        if ((kb & 3) == 1 && kb + 3 < g.KB) ask_scales(kb + 3);
+      } else {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((D - 2) * kLoads) : "memory");
+        load_scales(kb + D);
+      }
     });
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may reach LDS that is another workgroup's by then
@@ -225,7 +250,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
   // the registers they cost the L2 twelve times the requests.  Piece c (16 bytes) of row r lies at c ^ (r % kPieces).
   asm volatile("s_barrier" ::: "memory");  // all waves are past their last reads of the operands
   constexpr int kPieces = BN / 8;
-  static_assert(BM * BN * 2 <= 2 * kBuf && (kPieces & (kPieces - 1)) == 0, "the tile fits where the operands were");
+  static_assert(BM * BN * 2 <= D * kBuf && (kPieces & (kPieces - 1)) == 0, "the tile fits where the operands were");
 #pragma unroll
   for (int j = 0; j < NI; ++j)
 #pragma unroll
@@ -262,51 +287,54 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
 }
 
 // ---- few rows ----------------------------------------------------------------------------------
-// The weights are read once, straight into registers: a workgroup takes 16 of their rows against 16 MT
-// rows of a, its eight waves every eighth block of 128 columns, four blocks' loads in flight; the waves'
-// sums meet in LDS in wave order.
+// The weights are read once, straight into registers: a workgroup takes 16 of their rows against 16 MT rows of a,
+// its eight waves a stretch of the blocks each, kDepth blocks' loads in flight; the waves' sums meet in LDS in
+// wave order.  A lane takes the 16-byte pieces l / 16 and l / 16 + 4 of a row's 128 bytes, so that each load
+// instruction reads whole halves of lines.
 template <int MT, typename O>
 __global__ __launch_bounds__(512) void k_gemm8_rows(Gemm8Args g) {
-  constexpr int NW = 8, kDepth = MT > 2 ? 2 : 4;
+  constexpr int NW = 8, kDepth = 4;
   __shared__ f32x4 part[NW][MT][64];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, fr = lane & 15, fp = lane >> 4;
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
   const int64_t Kp = (int64_t)g.KB * kBlk;
   const int64_t nr = min(n0 + fr, g.N - 1);
-  const unsigned char* w = g.w + nr * Kp + fp * 32;
+  const unsigned char* w = g.w + nr * Kp + fp * 16;
   const unsigned char* ew = g.ew + nr * g.KB;
   const unsigned char* a[MT];
   const unsigned char* ea[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int64_t m = min(m0 + i * 16 + fr, g.M - 1);
-    a[i] = g.a + m * Kp + fp * 32;
+    a[i] = g.a + m * Kp + fp * 16;
     ea[i] = g.ea + m * g.KB;
   }
+  auto frag = [](const unsigned char* p) {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(p), hi = *reinterpret_cast<const i32x4*>(p + 64);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
   f32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int kb = wv; kb < g.KB; kb += NW * kDepth) {
+  const int per = (g.KB + NW - 1) / NW, k0 = min(wv * per, g.KB), k1 = min(k0 + per, g.KB);
+  for (int kb = k0; kb < k1; kb += kDepth) {
     i32x8 fw[kDepth], fa[kDepth][MT];
-    int sw[kDepth], sa[kDepth][MT];
+    unsigned sa[MT];
+    unsigned sw = scale4(ew, kb, g.KB);
 #pragma unroll
-    for (int d = 0; d < kDepth; ++d) {
-      const int k = kb + d * NW;
-      if (k < g.KB) {
-        fw[d] = *reinterpret_cast<const i32x8*>(w + (int64_t)k * kBlk);
-        sw[d] = ew[k];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          fa[d][i] = *reinterpret_cast<const i32x8*>(a[i] + (int64_t)k * kBlk);
-          sa[d][i] = ea[i][k];
-        }
-      }
-    }
+    for (int i = 0; i < MT; ++i) sa[i] = scale4(ea[i], kb, g.KB);
 #pragma unroll
     for (int d = 0; d < kDepth; ++d)
-      if (kb + d * NW < g.KB) {
+      if (kb + d < k1) {
+        fw[d] = frag(w + (int64_t)(kb + d) * kBlk);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i] = mfma8(fw[d], fa[d][i], acc[i], sw[d], sa[d][i]);
+        for (int i = 0; i < MT; ++i) fa[d][i] = frag(a[i] + (int64_t)(kb + d) * kBlk);
+      }
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d)
+      if (kb + d < k1) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i] = mfma8(fw[d], fa[d][i], acc[i], (int)(sw >> (8 * d)), (int)(sa[i] >> (8 * d)));
       }
   }
 #pragma unroll
@@ -320,20 +348,38 @@ __global__ __launch_bounds__(512) void k_gemm8_rows(Gemm8Args g) {
   }
 }
 
+// Which tile: the least of what each would take for a block of 128 columns, in units of 10 ns, from how many rounds
+// of workgroups its tiles fill the 256 compute units.  Measured (N = K = 4096 and neighbours): 64 x 64, two
+// workgroups a unit, 0.37 us a block up to one a unit, 0.61 a full round; 128 x 128, two a unit, 0.81 and 1.30;
+// 256 x 256, one a unit, 1.85 (8192 x 4096 x 8192 in 64 x 64 tiles takes twice its time, 512 x 4096 x 4096 in
+// 256 x 256 tiles 42 us against 20).
+int tile_of(int64_t t64, int64_t t128, int64_t t256) {
+  const int64_t c64 = t64 <= 256 ? 37 : (t64 + 511) / 512 * 61, c128 = t128 <= 256 ? 81 : (t128 + 511) / 512 * 130,
+                c256 = (t256 + 255) / 256 * 185;
+  return c64 <= c128 && c64 <= c256 ? 64 : c128 <= c256 ? 128 : 256;
+}
+
 template <typename O>
-void run_gemm8(const Gemm8Args& g, hipStream_t s) {
-  const auto tiles = [&](int bm, int bn) { return (int64_t)((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
-  if (g.M <= 16) {
-    hipLaunchKernelGGL((k_gemm8_rows<1, O>), dim3((g.N + 15) / 16, 1), dim3(512), 0, s, g);
+int run_gemm8(const Gemm8Args& g, hipStream_t s) {
+  const auto tiles = [&](int b) { return (int64_t)((g.M + b - 1) / b) * ((g.N + b - 1) / b); };
+  if (tiles(64) > 0x7fffffff) return dssm::report_error(DSSM_E_UNSUPPORTED, "blocks8_matmul: too many outputs");
+  const int tile = tile_of(tiles(64), tiles(128), tiles(256));
+  // Rows against rows where a is short, or where all the outputs are few: the waves of a workgroup share K (7 x 4096
+  // x 4096: 6.1 us against 11.2 in 64 x 64 tiles, 32 x 256 x 8192 10.0 against 18.1, 100 x 300 x 200 2.9 against
+  // 4.3); 32 rows at a time for 17 to 32 of them (32 x 4096 x 4096: 8.9 us, 10.7 sixteen at a time, 11.4 in tiles).
+  const int64_t n16 = (g.N + 15) / 16, m16 = (g.M + 15) / 16;
+  if (g.M <= 16 || n16 * m16 <= 256) {
+    hipLaunchKernelGGL((k_gemm8_rows<1, O>), dim3((unsigned)n16, (unsigned)m16), dim3(512), 0, s, g);
   } else if (g.M <= 32) {
-    hipLaunchKernelGGL((k_gemm8_rows<2, O>), dim3((g.N + 15) / 16, 1), dim3(512), 0, s, g);
-  } else if (g.M <= 64 || tiles(128, 128) < 64) {
-    hipLaunchKernelGGL((k_gemm8_rows<4, O>), dim3((g.N + 15) / 16, (g.M + 63) / 64), dim3(512), 0, s, g);
-  } else if (tiles(256, 256) < 128) {
-    hipLaunchKernelGGL((k_gemm8<2, 2, 2, 2, O>), dim3((unsigned)tiles(128, 128)), dim3(256), 0, s, g);
+    hipLaunchKernelGGL((k_gemm8_rows<2, O>), dim3((unsigned)n16, 1), dim3(512), 0, s, g);
+  } else if (tile == 64) {
+    hipLaunchKernelGGL((k_gemm8<2, 2, 1, 1, 4, O>), dim3((unsigned)tiles(64)), dim3(256), 0, s, g);
+  } else if (tile == 128) {
+    hipLaunchKernelGGL((k_gemm8<2, 2, 2, 2, 2, O>), dim3((unsigned)tiles(128)), dim3(256), 0, s, g);
   } else {
-    hipLaunchKernelGGL((k_gemm8<2, 4, 4, 2, O>), dim3((unsigned)tiles(256, 256)), dim3(512), 0, s, g);
+    hipLaunchKernelGGL((k_gemm8<2, 4, 4, 2, 2, O>), dim3((unsigned)tiles(256)), dim3(512), 0, s, g);
   }
+  return seq_status(hipGetLastError());
 }
 
 }  // namespace
@@ -359,7 +405,5 @@ extern "C" int dssm_blocks8_matmul(const void* a, const void* ascale, const void
   g.M = (int)M;
   g.N = (int)N;
   g.KB = (int)((K + kBlk - 1) / kBlk);
-  if (out_dtype == DSSM_BF16) run_gemm8<u16>(g, (hipStream_t)stream);
-  else run_gemm8<f16s>(g, (hipStream_t)stream);
-  return seq_status(hipGetLastError());
+  return out_dtype == DSSM_BF16 ? run_gemm8<u16>(g, (hipStream_t)stream) : run_gemm8<f16s>(g, (hipStream_t)stream);
 }
