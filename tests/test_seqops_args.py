@@ -86,8 +86,9 @@ def test_c_entries_refuse():
         F.dssm_embedding_lookup(0, L, 4, 4, 4, p, 0, 3, 1.0, p, L, 0),
         F.dssm_embedding_lookup(p, L, 3, 4, 4, p, 0, 3, 1.0, p, L, 0),
         F.dssm_embedding_lookup(p, 2, 4, 4, 4, p, 0, 3, 1.0, p, L, 0),
-        F.dssm_embedding_grad(p, B, 4, p, 0, 3, 4, 4, 1.0, p, p, 16, 0),
+        F.dssm_embedding_grad(p, B, 4, p, 0, 4000, 4, 4, 1.0, p, p, 16, 0),
         F.dssm_embedding_grad(p, B, 4, p, 0, 3, 4, 4, 1.0, p + 4, p, 1 << 20, 0),
+        F.dssm_embedding_grad(p, B, 3, p, 0, 3, 4, 4, 1.0, p, p, 1 << 20, 0),
         F.dssm_linear_recurrence(p, 8, 4, 0, 8, 4, B, 0, 0, 2, 2, 4, 0, p, 8, 4, p, 0, 0, 0, 0),
         F.dssm_linear_recurrence(p, 8, 4, p, 8, 4, 7, 0, 0, 2, 2, 4, 0, p, 8, 4, p, 0, 0, 0, 0),
         F.dssm_linear_recurrence(p, 0, 4, p, 0, 4, B, 0, 0, 1, 1 << 16, 4, 0, p, 0, 4, p, 0, 0, 0, 0),
