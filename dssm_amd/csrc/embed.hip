@@ -706,6 +706,7 @@ int run_grad(const void* dy, int dtype, int64_t lddy, const I* ids, int64_t n, i
     return f;
   };
   int grid = 0, side = 0;
+  if (g.spans > kMaxBlocks) return dssm::report_error(DSSM_E_UNSUPPORTED, "embedding_grad: too many ids");
   if (n == 0) {
     return seq_status(zero_bytes_async(dtable, (size_t)total * 4, s));
   } else if (one) {
@@ -768,7 +769,7 @@ extern "C" int dssm_embedding_lookup(const void* table, int dtype, int64_t ldt, 
   if (n == 0) return DSSM_OK;
   const int v = cols_of(E, 8), lg = lanes_log2(E, v);
   const int64_t rows = (int64_t)(256 >> lg) * kLookRows, blocks = (n + rows - 1) / rows;
-  if (blocks > 0x7fffffff) return dssm::report_error(DSSM_E_UNSUPPORTED, "embedding_lookup: too many ids");
+  if (blocks > kMaxBlocks) return dssm::report_error(DSSM_E_UNSUPPORTED, "embedding_lookup: too many ids");
   by_dtype(dtype, [&](auto t) {
     by_dtype(out_dtype, [&](auto o) {
       by_cols_of(v, [&](auto vec) {

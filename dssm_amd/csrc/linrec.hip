@@ -506,7 +506,7 @@ Cut cut_of(int64_t R, int T, int H, int dtype) {
 
 bool recur_dims_ok(int64_t R, int T, int H) {
   return R > 0 && T > 0 && H > 0 && T <= (1 << 28) && H <= (1 << 20) && R <= ((int64_t)1 << 31) &&
-         (R * H + 63) / 64 <= 0x7fffffff;
+         R * H <= ((int64_t)1 << 31);  // (a lane a state: a launch has fewer than 2^32 threads)
 }
 
 template <typename T, int V, bool FWD, bool W>

@@ -461,7 +461,7 @@ extern "C" int dssm_dequantize_blocks8(const void* q, const void* scale, int64_t
     return dssm::report_error(DSSM_E_INVALID, "dequantize_blocks8: bad argument (1 to 16384 columns, 16-byte aligned values)");
   if (rows == 0) return DSSM_OK;
   const int64_t units = rows * ((cols + 7) / 8);
-  if ((units + 255) / 256 > 0x7fffffff) return dssm::report_error(DSSM_E_UNSUPPORTED, "dequantize_blocks8: too many values");
+  if ((units + 255) / 256 > kMaxBlocks) return dssm::report_error(DSSM_E_UNSUPPORTED, "dequantize_blocks8: too many values");
   by_dtype(out_dtype, [&](auto tag) {
     using O = decltype(tag);
     hipLaunchKernelGGL(k_dequant<O>, dim3((unsigned)((units + 255) / 256)), dim3(256), 0, (hipStream_t)stream,

@@ -149,6 +149,8 @@ __device__ __forceinline__ float max16(float v) {
   return fmaxf(v, dpp_mov<0x140>(v));
 }
 
+constexpr int64_t kMaxBlocks = (1 << 24) - 1;  // workgroups of 256: a launch has fewer than 2^32 threads
+
 inline int seq_status(hipError_t e) {
   return e == hipSuccess ? DSSM_OK : report_error(DSSM_E_HIP, hipGetErrorString(e));
 }

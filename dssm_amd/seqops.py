@@ -157,8 +157,8 @@ def _recur_args(gate, cand, lens):
         raise TypeError("gate and cand must share a type")
     code = _code(gate.dtype, "gate")
     R, T, H = gate.shape
-    if T > 1 << 28 or H > 1 << 20 or R > 1 << 31:
-        raise ValueError("at most 2^31 rows, 2^28 steps and 2^20 channels")
+    if T > 1 << 28 or H > 1 << 20 or R * H > 1 << 31:
+        raise ValueError("at most 2^28 steps, 2^20 channels and 2^31 rows x channels")
     if lens is not None:
         if lens.dtype not in (torch.int32, torch.int64) or lens.dim() != 1 or lens.shape[0] != R:
             raise ValueError(f"lens must be int32 or int64 [{R}]")
@@ -249,8 +249,8 @@ def linear_recurrence_step(gate: torch.Tensor, cand: torch.Tensor, state: torch.
         raise TypeError("gate and cand must share a type")
     code = _code(gate.dtype, "gate")
     R, H = gate.shape
-    if H > 1 << 20 or R > 1 << 31:
-        raise ValueError("at most 2^31 rows and 2^20 channels")
+    if H > 1 << 20 or R * H > 1 << 31:
+        raise ValueError("at most 2^20 channels and 2^31 rows x channels")
     if state.dtype != torch.float32 or state.shape != gate.shape:
         raise ValueError(f"state must be float32 [{R} x {H}]")
     if (H > 1 and state.stride(1) != 1) or (R > 1 and state.stride(0) < H):

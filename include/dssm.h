@@ -716,7 +716,7 @@ int dssm_embedding_grad(const void* dy, int dtype, int64_t lddy, const void* ids
  * first.  h0 [R x H] fp32 or NULL (zeros); last [R x H] fp32: the state after the walk.  states (NULL for
  * inference): ceil(T / DSSM_RECUR_PIECE) x R x H floats, the state in front of every DSSM_RECUR_PIECE steps of
  * the walk, read by the backward.  ws: dssm_linear_recurrence_ws_bytes() bytes of any content (0: none
- * is needed, ws may be NULL); forward and backward need the same. */
+ * is needed, ws may be NULL); forward and backward need the same.  T <= 2^28, H <= 2^20, R * H <= 2^31. */
 #define DSSM_RECUR_PIECE 8
 size_t dssm_linear_recurrence_ws_bytes(int64_t R, int T, int H, int dtype);
 int dssm_linear_recurrence(const void* gate, int64_t gate_row, int64_t gate_time, const void* cand, int64_t cand_row,

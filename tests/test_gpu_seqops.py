@@ -72,7 +72,7 @@ def check_grad(device, dy, ids, V, scale=0.5):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,V,E", [(1, 1, 1), (2, 5, 3), (31, 3, 8), (32, 3, 8), (33, 1, 7), (64, 2, 16), (1000, 40, 100),
+@pytest.mark.parametrize("n,V,E", [(1, 1, 1), (2, 5, 3), (31, 3, 8), (32, 3, 8), (33, 1, 7), (64, 2, 16), (100, 1, 1), (1000, 40, 100),
                                    (4096, 700, 20), (4097, 700, 20), (5000, 1023, 9), (9000, 1024, 5), (12345, 70000, 12),
                                    (3, 1 << 21, 2)])
 def test_lookup_grad(device, n, V, E, dtype):
@@ -253,6 +253,13 @@ def test_recurrence_strides(device, dtype):
     same(odd[..., 1:H + 1], args[1], args[4], args[3].t().contiguous().t())
     cf = [x.permute(0, 2, 1).contiguous().permute(0, 2, 1) for x in (args[0], args[1], args[4])]  # channels apart
     same(cf[0], cf[1], cf[2], args[3])
+    # rows so far apart that a wave's offsets pass 32 bits
+    far = 40_000_000
+    away = [torch.zeros(far * (R - 1) + T * H, dtype=dtype, device=device).as_strided((R, T, H), (far, H, 1)) for _ in range(3)]
+    for x, y in zip(away, (args[0], args[1], args[4])):
+        x.copy_(y)
+    same(away[0], away[1], away[2], args[3])
+    del away
     # one gate for all rows
     h, _ = api.linear_recurrence(args[0][:1].expand(R, T, H), args[1])
     h2, _ = api.linear_recurrence(args[0][:1].repeat(R, 1, 1), args[1])
@@ -497,7 +504,8 @@ def product(a, w, bias, K):
 @pytest.mark.parametrize("out", [BF, F16])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 300, 128), (7, 17, 129), (16, 40, 1000), (17, 64, 2000), (33, 130, 257),
                                    (65, 300, 513), (64, 16, 4500), (200, 77, 640), (1100, 1030, 300), (257, 4100, 400),
-                                   (3000, 3001, 130)])
+                                   (3000, 3001, 130), (1500, 1500, 100), (1500, 1500, 1300), (200, 500, 3000),
+                                   (100, 300, 200), (3000, 3001, 1100)])
 def test_product(device, M, N, K, out):
     g = gen(M + N + K)
     a = api.quantize_blocks8((torch.randn(M, K, generator=g) * torch.exp(torch.randn(M, 1, generator=g))).to(device))
