@@ -155,15 +155,16 @@ struct SortLds {
 };
 
 // The whole sort of at most 4096 pairs in one workgroup: the digits' passes move the pairs through LDS.
+// (4 pairs a thread for 4000 ids: 22 us for the whole gradient, the same as many tiles' 23 for 5000; 16 a thread
+// for 16384: 45 us against 27.)
 constexpr int kOneSort = 4096;
 
-template <typename I>
+template <typename I, int kItems>
 __global__ __launch_bounds__(1024) void k_sort_one(const I* __restrict__ ids, int n, unsigned V, int bits, int passes,
                                                    uint2* __restrict__ pairs, Fill f) {
-  constexpr int kItems = kOneSort / 1024;
   __shared__ SortLds s;
-  __shared__ unsigned lk[kOneSort];
-  __shared__ unsigned short lp[kOneSort];
+  __shared__ unsigned lk[1024 * kItems];
+  __shared__ unsigned short lp[1024 * kItems];
   if ((int)blockIdx.x >= f.first) return fill_role(f, blockIdx.x - f.first, gridDim.x - f.first);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   unsigned k[kItems];
@@ -711,8 +712,8 @@ int run_grad(const void* dy, int dtype, int64_t lddy, const I* ids, int64_t n, i
     return seq_status(zero_bytes_async(dtable, (size_t)total * 4, s));
   } else if (one) {
     const Fill f = part_of(1, &grid, 1);
-    hipLaunchKernelGGL(k_sort_one<I>, dim3(grid), dim3(1024), 0, s, ids, (int)n, (unsigned)V, g.bits, g.passes,
-                       pairs[0], f);
+    auto kernel = n <= 1024 ? k_sort_one<I, 1> : k_sort_one<I, kOneSort / 1024>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(1024), 0, s, ids, (int)n, (unsigned)V, g.bits, g.passes, pairs[0], f);
   } else {
     const int tiles = (int)g.tiles;
     for (int q = 0; q < g.passes; ++q) {

@@ -136,13 +136,29 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
+        float y[8];
+        unsigned tie = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          // v rstd w with the product's rounding error and rstd's rest put back: a value next to a border of
-          // the 8-bit grid falls to the side that it is on
+          // v rstd w, with the product's rounding error and rstd's rest put back: rounded once
           const float p = v[k][i] * w[k][i], e = fmaf(v[k][i], w[k][i], -p);
-          v[k][i] = i < nv ? fmaf(p, rstd, fmaf(p, rest, e * rstd)) : 0.f;
+          y[i] = i < nv ? fmaf(p, rstd, fmaf(p, rest, e * rstd)) : 0.f;
+          tie |= (__float_as_uint(y[i]) & 0x7ffffu) == 0u;
         }
+        if (MODE == 1 && tie) {
+          // y that lies half way between two e4m3 values (these have their last 19 bits clear; so have zeros) may
+          // have got there by its own rounding: it moves to the side that the exact value is on
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float p = v[k][i] * w[k][i], e = fmaf(v[k][i], w[k][i], -p);
+            const float d = fmaf(p, rstd, -y[i]) + fmaf(p, rest, e * rstd);
+            const unsigned u = __float_as_uint(y[i]);
+            if (i < nv && (u & 0x7ffffu) == 0u && (u << 1) != 0u && (u << 1) < 0xff000000u && d != 0.f)
+              y[i] = __uint_as_float((d > 0.f) == (y[i] > 0.f) ? u + 1u : u - 1u);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[k][i] = y[i];
         if (MODE == 0 && nv > 0) st_row<T, 8>((T*)a.y + r * a.ldy + c, nv, v[k]);
       }
     }
