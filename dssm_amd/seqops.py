@@ -46,44 +46,47 @@ def _code(dtype: torch.dtype, what: str) -> int:
     return c
 
 
-def _on_gpu(first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
+# What a call costs on the host decides small ones (a few tokens): attributes are read once, and what is
+# looked up by name is kept.
+def _on_gpu(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The index of the device that all tensors are on."""
     dev = first.get_device()  # (-1: host memory)
     for t in others:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
     if dev < 0:
         raise ValueError("tensors must be on the GPU (the HIP path has no CPU fallback)")
-    return first.device
+    return dev
 
 
 _entries = {}
+_empty = torch.empty
+# the stream's handle itself: the wrapper object of torch.cuda.current_stream() costs as much as half a launch
+_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _call(dev: torch.device, name: str, *args):
+def _call(dev: int, name: str, *args):
     """The entry point on the device's current stream, with that device current."""
     f = _entries.get(name)
     if f is None:
         f = _entries[name] = getattr(_lib.load(), name)
-    # the handle itself: the wrapper object of torch.cuda.current_stream() costs as much as half a launch
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if dev.index == torch.cuda.current_device():
-        rc = f(*args, stream)
+    if dev == torch._C._cuda_getDevice():
+        rc = f(*args, _stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = f(*args, stream)
+            rc = f(*args, _stream(dev))
     if rc:
         _lib.check(rc, name)
 
 
 def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """x [..., cols] as [rows x cols] with neighbouring columns, and its row stride."""
-    cols = x.shape[-1]
     if x.dim() != 2:
-        x = x.reshape(-1, cols)
-    n = x.shape[0]
-    if (cols > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < cols):
-        x = x.contiguous()
-    return x, (x.stride(0) if n > 1 else cols)
+        x = x.reshape(-1, x.shape[-1])
+    (n, cols), (s0, s1) = x.shape, x.stride()
+    if (cols > 1 and s1 != 1) or (n > 1 and s0 < cols):
+        return x.contiguous(), cols
+    return x, (s0 if n > 1 else cols)
 
 
 def _vector(v: Optional[torch.Tensor], n: int, what: str) -> Optional[torch.Tensor]:
@@ -114,7 +117,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
     dev = _on_gpu(table, ids)
     V, E = table.shape
     table, ld = _rows(table)
-    out = torch.empty(*ids.shape, E, dtype=out_dtype, device=dev)
+    out = _empty(*ids.shape, E, dtype=out_dtype, device=dev)
     if ids.numel():
         _call(dev, "dssm_embedding_lookup", table.data_ptr(), code, ld, V, E, ids.data_ptr(),
               int(ids.dtype == torch.int64), ids.numel(), float(scale), out.data_ptr(), out_code)
@@ -137,8 +140,8 @@ def embedding_grad(dy: torch.Tensor, ids: torch.Tensor, nwords: int, scale: floa
                          "(fewer than 2^31 - 4096 ids, 1 to 2^30 - 1 words, 1 to 2^20 columns)")
     dev = _on_gpu(dy, ids)
     dy, ld = _rows(dy)
-    out = torch.empty(V, E, dtype=torch.float32, device=dev)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    out = _empty(V, E, dtype=torch.float32, device=dev)
+    ws = _empty(need, dtype=torch.uint8, device=dev)
     _call(dev, "dssm_embedding_grad", dy.data_ptr(), code, ld, ids.data_ptr(), int(ids.dtype == torch.int64), n, V, E,
           float(scale), out.data_ptr(), ws.data_ptr(), need)
     return out
@@ -151,12 +154,13 @@ def _steps(x: torch.Tensor) -> torch.Tensor:
 
 
 def _recur_args(gate, cand, lens):
-    if gate.dim() != 3 or gate.shape != cand.shape or gate.shape[2] == 0:
+    shape, dtype = gate.shape, gate.dtype
+    if len(shape) != 3 or cand.shape != shape or shape[2] == 0:
         raise ValueError("gate and cand must be [rows x steps x channels] alike")
-    if gate.dtype != cand.dtype:
+    if cand.dtype != dtype:
         raise TypeError("gate and cand must share a type")
-    code = _code(gate.dtype, "gate")
-    R, T, H = gate.shape
+    code = _code(dtype, "gate")
+    R, T, H = shape
     if T > 1 << 28 or H > 1 << 20 or R * H > 1 << 31:
         raise ValueError("at most 2^28 steps, 2^20 channels and 2^31 rows x channels")
     if lens is not None:
@@ -164,7 +168,7 @@ def _recur_args(gate, cand, lens):
             raise ValueError(f"lens must be int32 or int64 [{R}]")
         # (clamped before it is narrowed: a length past 2^31 means the whole row)
         lens = lens.contiguous() if lens.dtype == torch.int32 else lens.clamp(0, T).to(torch.int32)
-    return code, R, T, H, _steps(gate), _steps(cand), lens
+    return code, dtype, R, T, H, _steps(gate), _steps(cand), lens
 
 
 def _state(s: Optional[torch.Tensor], R: int, H: int, what: str) -> Optional[torch.Tensor]:
@@ -181,7 +185,7 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
 
 def _recur_ws(dev, R, T, H, code):
     need = int(_lib.load().dssm_linear_recurrence_ws_bytes(R, T, H, code))
-    return (torch.empty(need, dtype=torch.uint8, device=dev) if need else None), need
+    return (_empty(need, dtype=torch.uint8, device=dev) if need else None), need
 
 
 def linear_recurrence(gate: torch.Tensor, cand: torch.Tensor, lens: Optional[torch.Tensor] = None,
@@ -193,15 +197,15 @@ def linear_recurrence(gate: torch.Tensor, cand: torch.Tensor, lens: Optional[tor
     lens [R]: a row's steps, clamped to [0, T]; the steps behind them are not read, h is zero there and
     `last` is the state at the row's end (h0 for an empty row), as tf.nn.dynamic_rnn has it.  h0 [R x H]
     fp32 (default: zeros).  reverse: from each row's last step to its first, h at the steps' own places."""
-    code, R, T, H, gate, cand, lens = _recur_args(gate, cand, lens)
+    code, dtype, R, T, H, gate, cand, lens = _recur_args(gate, cand, lens)
     h0 = _state(h0, R, H, "h0")
     dev = _on_gpu(gate, cand, lens, h0)
-    h = torch.empty(R, T, H, dtype=gate.dtype, device=dev)
-    states = torch.empty(-(-T // _PIECE), R, H, dtype=torch.float32, device=dev) if save else None
+    h = _empty(R, T, H, dtype=dtype, device=dev)
+    states = _empty(-(-T // _PIECE), R, H, dtype=torch.float32, device=dev) if save else None
     if R == 0 or T == 0:
         last = torch.zeros(R, H, dtype=torch.float32, device=dev) if h0 is None else h0.clone()
         return (h, last, states) if save else (h, last)
-    last = torch.empty(R, H, dtype=torch.float32, device=dev)
+    last = _empty(R, H, dtype=torch.float32, device=dev)
     ws, need = _recur_ws(dev, R, T, H, code)
     _call(dev, "dssm_linear_recurrence", gate.data_ptr(), gate.stride(0), gate.stride(1), cand.data_ptr(), cand.stride(0),
           cand.stride(1), code, _ptr(lens), _ptr(h0), R, T, H, int(bool(reverse)), h.data_ptr(), T * H, H, last.data_ptr(),
@@ -216,7 +220,7 @@ def linear_recurrence_grad(gate: torch.Tensor, cand: torch.Tensor, states: torch
     dh [R x T x H] in the inputs' type (None: zero; not read behind a row's steps) and dlast [R x H] fp32
     (None: zero) -> (dgate, dcand [R x T x H] in the inputs' type, dh0 [R x H] fp32); dgate and dcand are
     zero behind a row's steps."""
-    code, R, T, H, gate, cand, lens = _recur_args(gate, cand, lens)
+    code, dtype, R, T, H, gate, cand, lens = _recur_args(gate, cand, lens)
     if states.dtype != torch.float32 or tuple(states.shape) != (-(-T // _PIECE), R, H) or not states.is_contiguous():
         raise ValueError("states must be what linear_recurrence(..., save=True) returned for these inputs")
     if dh is not None:
@@ -225,12 +229,12 @@ def linear_recurrence_grad(gate: torch.Tensor, cand: torch.Tensor, states: torch
         dh = _steps(dh)
     dlast = _state(dlast, R, H, "dlast")
     dev = _on_gpu(gate, cand, states, dh, dlast, lens)
-    dgate = torch.empty(R, T, H, dtype=gate.dtype, device=dev)
-    dcand = torch.empty(R, T, H, dtype=gate.dtype, device=dev)
+    dgate = _empty(R, T, H, dtype=dtype, device=dev)
+    dcand = _empty(R, T, H, dtype=dtype, device=dev)
     if R == 0 or T == 0:
         dh0 = torch.zeros(R, H, dtype=torch.float32, device=dev) if dlast is None else dlast.clone()
         return dgate, dcand, dh0
-    dh0 = torch.empty(R, H, dtype=torch.float32, device=dev)
+    dh0 = _empty(R, H, dtype=torch.float32, device=dev)
     ws, need = _recur_ws(dev, R, T, H, code)
     dr, dt = (0, 0) if dh is None else (dh.stride(0), dh.stride(1))
     _call(dev, "dssm_linear_recurrence_bwd", gate.data_ptr(), gate.stride(0), gate.stride(1), cand.data_ptr(),
@@ -243,25 +247,27 @@ def linear_recurrence_step(gate: torch.Tensor, cand: torch.Tensor, state: torch.
     """One step of running states: state [R x H] fp32 moves on in place, the new state in the inputs' type
     is returned.  gate, cand [R x H] (rows of any stride); state's rows must not overlap each other or the
     inputs."""
-    if gate.dim() != 2 or gate.shape != cand.shape or gate.shape[1] == 0:
+    shape, dtype = gate.shape, gate.dtype
+    if len(shape) != 2 or cand.shape != shape or shape[1] == 0:
         raise ValueError("gate and cand must be [rows x channels] alike")
-    if gate.dtype != cand.dtype:
+    if cand.dtype != dtype:
         raise TypeError("gate and cand must share a type")
-    code = _code(gate.dtype, "gate")
-    R, H = gate.shape
+    code = _code(dtype, "gate")
+    R, H = shape
     if H > 1 << 20 or R * H > 1 << 31:
         raise ValueError("at most 2^20 channels and 2^31 rows x channels")
-    if state.dtype != torch.float32 or state.shape != gate.shape:
+    if state.dtype != torch.float32 or state.shape != shape:
         raise ValueError(f"state must be float32 [{R} x {H}]")
-    if (H > 1 and state.stride(1) != 1) or (R > 1 and state.stride(0) < H):
+    lds, inner = state.stride()
+    if (H > 1 and inner != 1) or (R > 1 and lds < H):
         raise ValueError("state's channels must be neighbours and its rows apart: it is updated in place")
     dev = _on_gpu(gate, cand, state)
     gate, ldg = _rows(gate)
     cand, ldc = _rows(cand)
-    h = torch.empty(R, H, dtype=gate.dtype, device=dev)
+    h = _empty(R, H, dtype=dtype, device=dev)
     if R:
-        _call(dev, "dssm_linear_recurrence_step", gate.data_ptr(), ldg, cand.data_ptr(), ldc, code, state.data_ptr(),
-              state.stride(0), h.data_ptr(), H, R, H)
+        _call(dev, "dssm_linear_recurrence_step", gate.data_ptr(), ldg, cand.data_ptr(), ldc, code, state.data_ptr(), lds,
+              h.data_ptr(), H, R, H)
     return h
 
 
@@ -286,12 +292,12 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     cols = x.shape[-1]
     x2, ldx = _rows(x)
     rows = x2.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev)
+    y = _empty(x.shape, dtype=x.dtype, device=dev)
+    rstd = _empty(rows, dtype=torch.float32, device=dev)
     r2, ldr, s = None, 0, x
     if residual is not None:
         r2, ldr = _rows(residual)
-        s = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        s = _empty(x.shape, dtype=x.dtype, device=dev)
     if rows:
         _call(dev, "dssm_rms_norm", x2.data_ptr(), ldx, _ptr(r2), ldr, weight.data_ptr(), rows, cols, code, float(eps),
               y.data_ptr(), cols, 0 if r2 is None else s.data_ptr(), cols, rstd.data_ptr())
@@ -315,12 +321,12 @@ def rms_norm_grad(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor, rstd:
     s2, lds = _rows(s)
     ds2, ldds = (None, 0) if ds is None else _rows(ds)
     dev = _on_gpu(dy, s, weight, rstd, ds)
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
-    dw = torch.empty(cols, dtype=torch.float32, device=dev)
+    dx = _empty(dy.shape, dtype=dy.dtype, device=dev)
+    dw = _empty(cols, dtype=torch.float32, device=dev)
     if not rows:
         return dx, dw.zero_()
     need = int(_lib.load().dssm_rms_norm_bwd_ws_bytes(rows, cols))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = _empty(need, dtype=torch.uint8, device=dev)
     _call(dev, "dssm_rms_norm_bwd", dy2.data_ptr(), lddy, s2.data_ptr(), lds, weight.data_ptr(), rstd.data_ptr(), _ptr(ds2),
           ldds, rows, cols, code, dx.data_ptr(), cols, dw.data_ptr(), ws.data_ptr(), need)
     return dx, dw
@@ -329,8 +335,8 @@ def rms_norm_grad(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor, rstd:
 # ---- 8-bit block form --------------------------------------------------------------------------------
 def _empty8(rows: int, cols: int, dev) -> Blocks8:
     kb = -(-cols // BLOCK)
-    return Blocks8(torch.empty(rows, kb * BLOCK, dtype=torch.float8_e4m3fn, device=dev),
-                   torch.empty(rows, kb, dtype=torch.float8_e8m0fnu, device=dev), cols)
+    return Blocks8(_empty(rows, kb * BLOCK, dtype=torch.float8_e4m3fn, device=dev),
+                   _empty(rows, kb, dtype=torch.float8_e8m0fnu, device=dev), cols)
 
 
 def _check8(b: Blocks8, what: str) -> int:
@@ -356,7 +362,7 @@ def rms_norm_blocks8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
     r2, ldr, s = None, 0, x
     if residual is not None:
         r2, ldr = _rows(residual)
-        s = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        s = _empty(x.shape, dtype=x.dtype, device=dev)
     if rows:
         _call(dev, "dssm_rms_norm_blocks8", x2.data_ptr(), ldx, _ptr(r2), ldr, weight.data_ptr(), rows, cols, code, float(eps),
               y.q.data_ptr(), y.scale.data_ptr(), 0 if r2 is None else s.data_ptr(), cols, 0)
@@ -387,7 +393,7 @@ def dequantize_blocks8(b: Blocks8, dtype: torch.dtype = torch.float32) -> torch.
     if b.cols > MAX_NORM_COLS:
         raise ValueError(f"b must have 1 to {MAX_NORM_COLS} columns")
     dev = _on_gpu(b.q, b.scale)
-    out = torch.empty(rows, b.cols, dtype=dtype, device=dev)
+    out = _empty(rows, b.cols, dtype=dtype, device=dev)
     if rows:
         _call(dev, "dssm_dequantize_blocks8", b.q.data_ptr(), b.scale.data_ptr(), rows, b.cols, out.data_ptr(), b.cols, code)
     return out
@@ -409,7 +415,7 @@ def blocks8_matmul(a: Blocks8, w: Blocks8, bias: Optional[torch.Tensor] = None,
         raise ValueError("at most 2^28 rows, 2^24 outputs and 2^22 columns")
     bias = _vector(bias, N, "bias")
     dev = _on_gpu(a.q, a.scale, w.q, w.scale, bias)
-    out = torch.empty(M, N, dtype=dtype, device=dev)
+    out = _empty(M, N, dtype=dtype, device=dev)
     if M and N:
         _call(dev, "dssm_blocks8_matmul", a.q.data_ptr(), a.scale.data_ptr(), w.q.data_ptr(), w.scale.data_ptr(), M, N, a.cols,
               _ptr(bias), out.data_ptr(), N, code)

@@ -118,3 +118,12 @@ def test_nothing_to_do_is_no_error():
     assert lib.dssm_rms_norm(0, 4, 0, 0, p, 0, 4, 0, 1e-6, 0, 4, 0, 0, 0, 0) == 0
     assert lib.dssm_quantize_blocks8(0, 4, 0, 4, 0, 0, 0, 0) == 0
     assert lib.dssm_blocks8_matmul(0, 0, 0, 0, 0, 2, 4, 0, 0, 2, _lib.DSSM_BF16, 0) == 0
+
+
+def test_the_states_pieces_are_the_librarys():
+    import os
+    import re
+
+    from dssm_amd import seqops
+    head = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "dssm.h")
+    assert int(re.search(r"#define DSSM_RECUR_PIECE (\d+)", open(head).read()).group(1)) == seqops._PIECE
