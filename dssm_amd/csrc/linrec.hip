@@ -482,7 +482,9 @@ __global__ __launch_bounds__(256) void k_recur_step(const T* __restrict__ gate, 
 // How the work is cut.  `waves`: waves of 64 lanes that the channels alone give.  From 1024 on (one for each SIMD)
 // a wave walks its row alone; below it, four or eight share the time of a workgroup's channels, and where even
 // that leaves fewer than 2048 waves, time is cut into segments until there are 4096 (2 x 65537 x 512: 140 us;
-// 181 with 2048, 154 with 8192), of two rounds of pieces at least.
+// 181 with 2048, 154 with 8192), of two rounds of pieces at least.  Up to four rounds stay one launch, whose rounds cost
+// less than a second launch's start (8 x 128 bf16: 133 steps 8.4 and 11.6 us, 11.8 and 15.4 cut; 256 steps 10.4 and
+// 16.4, 12.0 and 15.6 cut; 512 steps 18.4 and 29.7, 12.1 and 15.7 cut).
 struct Cut {
   int V, NW, S, L;
 };
@@ -497,7 +499,7 @@ Cut cut_of(int64_t R, int T, int H, int dtype) {
   if (waves < 1024 && pieces > 1) {
     c.NW = pieces >= 5 ? 8 : 4;
     const int64_t want = 4096 / (waves * c.NW);
-    if (want >= 2) c.S = (int)std::min<int64_t>(want, (pieces + 2 * c.NW - 1) / (2 * c.NW));
+    if (want >= 2 && pieces > 4 * c.NW) c.S = (int)std::min<int64_t>(want, (pieces + 2 * c.NW - 1) / (2 * c.NW));
   }
   const int round = c.NW * kPiece, per = (T + c.S - 1) / c.S;
   c.L = (per + round - 1) / round * round;
