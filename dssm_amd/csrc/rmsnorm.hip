@@ -12,13 +12,14 @@
 // block of 128 columns, so a block's scale is four DPP steps away.  A workgroup stays for many rows, its weights in
 // registers, with the next row's loads behind the current one's arithmetic.
 //
-// Measured: 196608 x 256 bf16 with a residual 85 us forward, 78 + 6 backward (4.7 TB/s of 403 MB each way, a large
-// copy's rate; one workgroup for every four rows took 117 and 119); 24571 x 1024 to the 8-bit form 35 us (5.0 TB/s),
-// its values back in bf16 16.5 us (4.6 TB/s).
+// Measured: 196608 x 256 bf16 with a residual 68 us forward, 83 + 5 backward (403 MB each way: 5.9 and 4.6 TB/s, the
+// forward's inputs in part still cached; one workgroup for every four rows took 117 and 119); 24571 x 1024 to the
+// 8-bit form 35 us (5.0 TB/s), its values back in bf16 14 us (5.4 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "seq.h"
 
@@ -87,25 +88,26 @@ struct NormArgs {
 // MODE 0: y in T; 1: y in the 8-bit form; 2: x itself in the 8-bit form (no norm).
 // A workgroup walks rows blockIdx.x * kRows + i * gridDim.x * kRows with the weights in registers and the next
 // rows' loads in flight behind the current ones' arithmetic.
-template <typename T, int NT, int K, int MODE>
+template <typename T, int NT, int K, int MODE, bool R>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
   constexpr int kRows = NT < 256 ? 256 / NT : 1;
   __shared__ double red[16];
   const int l = threadIdx.x % NT;
   const int64_t step = (int64_t)gridDim.x * kRows;
+  const bool whole = a.cols >= 8;
   float w[K][8];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (k * NT + l) * 8, nv = a.cols - c;
     if (MODE != 2 && nv > 0) ld_row<float, 8>(a.w + c, nv, w[k]);
   }
-  Ask<T> x[K], b[K];
+  Ask<T, R> x[K], b[K];
   auto ask = [&](int64_t r) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * NT + l) * 8, nv = r < a.rows ? a.cols - c : 0;
-      x[k].ask((const T*)a.x + r * a.ldx + c, nv);
-      if (MODE != 2 && a.res) b[k].ask((const T*)a.res + r * a.ldres + c, nv);
+      x[k].ask((const T*)a.x + r * a.ldx + c, nv, whole);
+      if (MODE != 2 && a.res) b[k].ask((const T*)a.res + r * a.ldres + c, nv, whole);
     }
   };
   int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / NT;
@@ -117,10 +119,10 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
-      x[k].take((const T*)a.x + r * a.ldx + c, nv, v[k]);
+      x[k].take((const T*)a.x + r * a.ldx + c, nv, whole, v[k]);
       if (MODE != 2 && a.res) {
         float t[8];
-        b[k].take((const T*)a.res + r * a.ldres + c, nv, t);
+        b[k].take((const T*)a.res + r * a.ldres + c, nv, whole, t);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[k][i] = ld1(st1<T>(v[k][i] + t[i]));
       }
@@ -129,8 +131,6 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
     if constexpr (MODE != 2) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
-        if (a.s && nv > 0) st_row<T, 8>((T*)a.s + r * a.lds + c, nv, v[k]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum = fmaf(v[k][i], v[k][i], sum);
       }
@@ -141,6 +141,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
+        // (s may be x or residual: it is stored behind the row sum, when no thread reads them any more)
+        if (a.s && nv > 0) st_row<T, 8, R>((T*)a.s + r * a.lds + c, nv, v[k]);
         float y[8];
         unsigned tie = 0;
 #pragma unroll
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[k][i] = y[i];
-        if (MODE == 0 && nv > 0) st_row<T, 8>((T*)a.y + r * a.ldy + c, nv, v[k]);
+        if (MODE == 0 && nv > 0) st_row<T, 8, R>((T*)a.y + r * a.ldy + c, nv, v[k]);
       }
     }
     if constexpr (MODE != 0) {
@@ -186,27 +188,28 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
 
 // Backward.  A workgroup walks rows blockIdx.x * kRows + i * gridDim.x * kRows and keeps its share of dw in
 // registers; its rows' slots meet in LDS at the end and the workgroup leaves one partial row.
-template <typename T, int NT, int K>
+template <typename T, int NT, int K, bool R>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_bwd(NormArgs a) {
   constexpr int kRows = NT < 256 ? 256 / NT : 1;
   __shared__ float red[16];
+  // the next row's loads in flight behind this one's arithmetic, but where 1024 threads hold 16 columns each: their
+  // 128 registers take no second row (16384 x 4096 bf16 110 us; 191 with both, which spills)
+  constexpr bool kAhead = NT * K < 2048;
   __shared__ float slot[kRows > 1 ? kRows : 1][kRows > 1 ? NT * 8 + 4 : 1];
   const int l = threadIdx.x % NT, g = threadIdx.x / NT;
   float w[K][8], dw[K][8];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (k * NT + l) * 8, nv = a.cols - c;
-    if (nv > 0) {
-      ld_row<float, 8>(a.w + c, nv, w[k]);
-    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[k][i] = 0.f;
-    }
+    for (int i = 0; i < 8; ++i) w[k][i] = 0.f;
+    if (nv > 0) ld_row<float, 8>(a.w + c, nv, w[k]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[k][i] = 0.f;
   }
   const int64_t step = (int64_t)gridDim.x * kRows;
-  Ask<T> as[K], ad[K], ax[K];
+  const bool whole = a.cols >= 8;
+  Ask<T, R> as[K], ad[K], ax[K];
   float arstd = 0.f;
   auto ask = [&](int64_t r) {
     const bool in = r < a.rows;
@@ -214,31 +217,36 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_bwd(NormArgs a) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
-      as[k].ask((const T*)a.s_in + r * a.lds + c, nv);
-      ad[k].ask((const T*)a.dy + r * a.lddy + c, nv);
-      if (a.ds) ax[k].ask((const T*)a.ds + r * a.ldds + c, nv);
+      as[k].ask((const T*)a.s_in + r * a.lds + c, nv, whole);
+      ad[k].ask((const T*)a.dy + r * a.lddy + c, nv, whole);
+      if (a.ds) ax[k].ask((const T*)a.ds + r * a.ldds + c, nv, whole);
     }
   };
   int64_t r = (int64_t)blockIdx.x * kRows + g;
-  ask(r);
+  if constexpr (kAhead) ask(r);
   for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < a.rows; r0 += step, r += step) {
     const bool in = r < a.rows;
+    if constexpr (!kAhead) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) as[k] = ad[k] = ax[k] = Ask<T, R>{};
+      ask(r);
+    }
     const float rstd = arstd;
     float n[K][8], d[K][8], o[K][8], sum = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
-      as[k].take((const T*)a.s_in + r * a.lds + c, nv, n[k]);
-      ad[k].take((const T*)a.dy + r * a.lddy + c, nv, d[k]);
-      if (a.ds) ax[k].take((const T*)a.ds + r * a.ldds + c, nv, o[k]);
+      as[k].take((const T*)a.s_in + r * a.lds + c, nv, whole, n[k]);
+      ad[k].take((const T*)a.dy + r * a.lddy + c, nv, whole, d[k]);
+      if (a.ds) ax[k].take((const T*)a.ds + r * a.ldds + c, nv, whole, o[k]);
       else
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[k][i] = 0.f;
     }
     // (the tails of an element-by-element read are in hand here too: dx may be dy or ds)
-    ask(r + step);
+    if constexpr (kAhead) ask(r + step);
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         n[k][i] = in ? n[k][i] * rstd : 0.f;
@@ -246,13 +254,14 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_bwd(NormArgs a) {
         d[k][i] *= w[k][i];
         sum = fmaf(d[k][i], n[k][i], sum);
       }
+    }
     const float mean = row_sum<NT, float>(sum, red) / (float)a.cols;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[k][i] = fmaf(rstd, d[k][i] - n[k][i] * mean, o[k][i]);
-      if (nv > 0) st_row<T, 8>((T*)a.dx + r * a.lddx + c, nv, o[k]);
+      if (nv > 0) st_row<T, 8, R>((T*)a.dx + r * a.lddx + c, nv, o[k]);
     }
   }
   float* out = a.part + (int64_t)blockIdx.x * a.cols;
@@ -288,7 +297,13 @@ __global__ __launch_bounds__(1024) void k_norm_dw(const float* __restrict__ part
   const int per = (blocks + 63) / 64, b0 = min(t * per, blocks), b1 = min(b0 + per, blocks);
   float v = 0.f;
   if (c < cols)
-    for (int b = b0; b < b1; ++b) v += part[(int64_t)b * cols + c];
+    for (int b = b0; b < b1; b += 8) {  // eight loads in flight
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = b + i < b1 ? part[(int64_t)(b + i) * cols + c] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += x[i];
+    }
   red[t][j] = v;
   __syncthreads();
   if (t == 0 && c < cols) {
@@ -325,18 +340,24 @@ __global__ __launch_bounds__(256) void k_dequant(const unsigned char* __restrict
 }
 
 // Threads a row: the fewest that hold it, but a whole workgroup for wide rows, whose wave would keep too
-// few loads in flight.
-template <typename F>
+// few loads in flight.  From 4097 to 8192 columns the forward takes two of 512 threads to a compute unit (8192 x 4100
+// bf16 54 us, 70 with 1024 threads of 8 columns; 4096 x 8192 46 either way), the backward, whose registers let only
+// one stay, 1024 (58 and 73).
+template <bool FWD, typename F>
 void by_cols(int cols, F&& f) {
   using std::integral_constant;
-  if (cols <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-  else if (cols <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
-  else if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-  else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-  else if (cols <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-  else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-  else if (cols <= 8192) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
-  else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+  auto go = [&](auto ragged) {
+    if (cols <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 1>{}, ragged);
+    else if (cols <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 1>{}, ragged);
+    else if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{}, ragged);
+    else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 2>{}, ragged);
+    else if (cols <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{}, ragged);
+    else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 2>{}, ragged);
+    else if (cols <= 8192) f(integral_constant<int, FWD ? 512 : 1024>{}, integral_constant<int, FWD ? 2 : 1>{}, ragged);
+    else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{}, ragged);
+  };
+  if (cols % 8) go(std::true_type{});
+  else go(std::false_type{});
 }
 
 bool norm_dims_ok(int64_t rows, int cols) {
@@ -348,17 +369,22 @@ template <int MODE>
 void run_norm(const NormArgs& a, int dtype, hipStream_t s) {
   by_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
-    by_cols(a.cols, [&](auto nt, auto kk) {
+    by_cols<true>(a.cols, [&](auto nt, auto kk, auto ragged) {
       constexpr int NT = decltype(nt)::value, K = decltype(kk)::value, rows = NT < 256 ? 256 / NT : 1;
-      const int64_t blocks = std::min<int64_t>((a.rows + rows - 1) / rows, NT < 1024 ? 2048 : 512);
-      hipLaunchKernelGGL((k_norm<T, NT, K, MODE>), dim3((unsigned)blocks), dim3(NT < 256 ? 256 : NT), 0, s, a);
+      const int64_t blocks = std::min<int64_t>((a.rows + rows - 1) / rows, NT < 512 ? 2048 : NT < 1024 ? 1024 : 512);
+      hipLaunchKernelGGL((k_norm<T, NT, K, MODE, decltype(ragged)::value>), dim3((unsigned)blocks), dim3(NT < 256 ? 256 : NT), 0, s, a);
     });
   });
 }
-constexpr int kBwdBlocks = 1024;  // partial rows of dw at most
+// Workgroups of the backward, each of which leaves a partial row of dw.  Above 4096 columns one of 1024 threads fills a
+// compute unit: 256 (4096 x 8192 bf16 46 us; 67 with 1024 of them).  Below, 512, whose fewer partial rows are worth
+// more than the waves (8192 x 1024 bf16 17.8 us, 20.2 with 1024; 16384 x 4096 107 and 126), but 1024 for narrow
+// rows (196608 x 64 bf16 21 us, 23 with 512) and for ragged ones, whose groups take more instructions (16384 x 1191
+// 40 and 59).  A row at a time: at least two rows each (512 x 4096 11.8 us, 15.1 with one).
 int bwd_blocks(int64_t rows, int cols) {
-  const int per = cols <= 128 ? 16 : cols <= 256 ? 8 : cols <= 1024 ? 4 : 1;  // rows a workgroup takes at once
-  return (int)std::max<int64_t>(1, std::min<int64_t>(kBwdBlocks, (rows + per - 1) / per));
+  const int per = cols <= 128 ? 16 : cols <= 256 ? 8 : cols <= 1024 ? 4 : 2;  // rows a workgroup takes at least
+  const int most = cols > 4096 ? 256 : cols <= 128 || cols % 8 ? 1024 : 512;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(most, (rows + per - 1) / per));
 }
 
 }  // namespace
@@ -448,9 +474,9 @@ extern "C" int dssm_rms_norm_bwd(const void* dy, int64_t lddy, const void* s, in
   const int blocks = bwd_blocks(rows, cols);
   by_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
-    by_cols(cols, [&](auto nt, auto kk) {
+    by_cols<false>(cols, [&](auto nt, auto kk, auto ragged) {
       constexpr int NT = decltype(nt)::value, K = decltype(kk)::value;
-      hipLaunchKernelGGL((k_norm_bwd<T, NT, K>), dim3(blocks), dim3(NT < 256 ? 256 : NT), 0, st, a);
+      hipLaunchKernelGGL((k_norm_bwd<T, NT, K, decltype(ragged)::value>), dim3(blocks), dim3(NT < 256 ? 256 : NT), 0, st, a);
     });
   });
   hipLaunchKernelGGL(k_norm_dw, dim3((cols + 15) / 16), dim3(1024), 0, st, (const float*)ws, blocks, cols, dweight);

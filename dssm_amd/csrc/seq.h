@@ -54,13 +54,27 @@ __device__ __forceinline__ void ld_row(const T* p, int n, float (&x)[V]) {
     for (int i = 0; i < V; ++i) x[i] = i < n ? ld1(p[i]) : 0.f;
   }
 }
-template <typename T, int V>
+// (by value: a choice between two array elements would put the array into memory)
+__device__ __forceinline__ float pick(bool c, float a, float b) { return c ? a : b; }
+template <typename T, int V, bool R = true>
 __device__ __forceinline__ void st_row(T* p, int n, const float (&x)[V]) {
   if (n >= V) {
     Pack<T, V> r;
 #pragma unroll
     for (int i = 0; i < V; ++i) r.v[i] = st1<T>(x[i]);
     stv<T, V>(p, r);
+  } else if constexpr (!R) {
+  } else if constexpr (V == 8) {  // four, two and one of them: three stores at most
+    if (n <= 0) return;
+    Pack<T, 4> a;
+    Pack<T, 2> b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a.v[i] = st1<T>(x[i]);
+    if (n & 4) stv<T, 4>(p, a);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) b.v[i] = st1<T>(pick(n & 4, x[i + 4], x[i]));
+    if (n & 2) stv<T, 2>(p + (n & 4), b);
+    if (n & 1) p[n - 1] = st1<T>(pick(n & 4, pick(n & 2, x[6], x[4]), pick(n & 2, x[2], x[0])));
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -69,21 +83,32 @@ __device__ __forceinline__ void st_row(T* p, int n, const float (&x)[V]) {
 }
 
 // The same load in two steps, so that a kernel asks for all it needs before it waits for any: ask() issues a
-// whole group's access and does not look at it, take() converts (a ragged group is read element by element
-// there: only the last lane of a row whose width is no multiple of 8 has one).
-template <typename T>
+// whole group's access and does not look at it, take() converts.  A ragged group (only the last one of a row whose
+// width is no multiple of 8) asks for the row's last eight elements, its neighbour's among them, and take() moves its
+// own down: element by element the row's end would wait for memory once more (44295 x 1191 bf16 forward 170 us and
+// 106 so, backward 256 and 114).  `whole`: the row has eight elements.  R false: no group is ragged, and the code
+// for them, which costs short launches 0.3 us, is left out.
+template <typename T, bool R>
 struct Ask {
   Pack<T, 8> r;
-  __device__ __forceinline__ void ask(const T* p, int n) {
-    if (n >= 8) r = ldv<T, 8>(p);
+  __device__ __forceinline__ void ask(const T* p, int n, bool whole) {
+    const T* q = !R || n >= 8 ? p : p + n - 8;
+    if (n > (R && whole ? 0 : 7)) r = ldv<T, 8>(q);
   }
-  __device__ __forceinline__ void take(const T* p, int n, float (&x)[8]) const {
-    if (n >= 8) {
+  __device__ __forceinline__ void take(const T* p, int n, bool whole, float (&x)[8]) const {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = ld1(r.v[i]);
-    } else {
+    for (int i = 0; i < 8; ++i) x[i] = ld1(r.v[i]);
+    if (n < 8) {
+      if (R && whole && n > 0) {
+        const int down = 8 - n;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = i < n ? ld1(p[i]) : 0.f;
+        for (int d = 4; d; d >>= 1)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = down & d ? (i + d < 8 ? x[i + d] : 0.f) : x[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = R && i < n ? ld1(p[i]) : 0.f;
+      }
     }
   }
 };

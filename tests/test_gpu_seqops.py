@@ -4,7 +4,7 @@ where they are used; `stored` is the one rounding into the output's type."""
 import pytest
 import torch
 
-from dssm_amd import api
+from dssm_amd import _lib, api, seqops
 from tests import seqops_ref as ref
 
 pytestmark = pytest.mark.gpu
@@ -161,7 +161,7 @@ def check_recurrence(device, gate, cand, lens, h0, reverse, g, grad=True):
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("R,T,H,dtype", [(1, 1, 1, F32), (3, 1, 5, BF), (2, 16, 6, F16), (5, 17, 33, BF), (4, 40, 64, BF),
                                          (3, 63, 10, F32), (2, 129, 130, F16), (600, 33, 128, BF), (2100, 18, 64, F32),
-                                         (1050, 20, 65, F16), (3, 300, 7, BF), (1, 1029, 3, F32), (2, 2500, 20, BF)])
+                                         (1050, 20, 65, F16), (2, 256, 6, BF), (2, 257, 6, F32), (3, 300, 7, BF), (1, 1029, 3, F32), (2, 2500, 20, BF)])
 def test_recurrence(device, R, T, H, dtype, reverse):
     gate, cand, lens, h0, g = inputs(R, T, H, dtype, R + T + H)
     check_recurrence(device, gate, cand, lens, h0, reverse, g)
@@ -435,6 +435,64 @@ def test_norm_shapes_and_strides(device):
     # a column of all rows: one column, rows far apart
     col = x.view(15, 90)[:, 4:5]
     near(api.rms_norm(col, w[:1])[0], ref.norm(col.cpu(), w[:1].cpu(), None, 1e-6)[0], 0.02)
+
+
+def test_norm_ragged_rows(device):
+    """Every width of a ragged end, in rows whose surroundings are NaN: what lies beside a row is not used."""
+    g = gen(5)
+    for dtype in TYPES:
+        for cols in list(range(1, 25)) + [133, 262, 1030, 4099]:
+            x, dy = torch.randn(19, cols, generator=g).to(dtype), torch.randn(19, cols, generator=g).to(dtype)
+            w = torch.rand(cols, generator=g) + 0.5
+            base = torch.full((2, 19, cols + 11), float("nan"), dtype=dtype, device=device)
+            xs, dys = base[0, :, 5:5 + cols], base[1, :, 5:5 + cols]
+            xs.copy_(x)
+            dys.copy_(dy)
+            y, s, rstd = api.rms_norm(xs, w.to(device), dys)
+            eps = float(torch.tensor(1e-6))
+            wy, ws, wr = ref.norm(x, w, dy, eps)
+            assert torch.equal(s.cpu(), ws)
+            rounded(y, wy, NORM * wy.abs())
+            dx, dw = api.rms_norm_grad(dys, s, w.to(device), rstd, xs)
+            wx, wdw, mx, mw = ref.norm_grad(dy, ws, w, wr, x)
+            rounded(dx, wx, 2 * NORM * mx)
+            near(dw, wdw, 59 * U * mw)
+            y8, _ = api.rms_norm_blocks8(xs, w.to(device), dys)
+            check_blocks(y8, wy, NORM * wy.abs())
+
+
+# rows enough that a workgroup walks several, at every number of threads a row; the outputs over the inputs, as the
+# C entry points allow: s over x or the residual, dx over dy or ds
+@pytest.mark.parametrize("rows,cols,dtype", [(40000, 24, BF), (40001, 21, F16), (9000, 200, F32), (9001, 501, BF),
+                                             (8500, 1000, F16), (2500, 2041, BF), (2200, 4096, BF), (1100, 4103, F32),
+                                             (1500, 8192, F16), (600, 8203, F32), (600, 12000, BF), (530, 16384, F32)])
+def test_norm_many_rows_in_place(device, rows, cols, dtype):
+    g = torch.Generator(device).manual_seed(rows)
+    code = seqops._code(dtype, "x")
+    x, res, dy, ds = (torch.randn(rows, cols, generator=g, device=device).to(dtype) for _ in range(4))
+    w = torch.rand(cols, generator=g, device=device) + 0.5
+    y, s, rstd = api.rms_norm(x, w, res)
+    dx, dw = api.rms_norm_grad(dy, s, w, rstd, ds)
+    pick = torch.unique(torch.cat([torch.arange(0, rows, max(rows // 40, 1)), torch.arange(rows - 3, rows)]))
+    wy, ws, wr = ref.norm(x[pick].cpu(), w.cpu(), res[pick].cpu(), float(torch.tensor(1e-6)))
+    assert torch.equal(s[pick].cpu(), ws)
+    rounded(y[pick], wy, NORM * wy.abs())
+    wx, _, mx, _ = ref.norm_grad(dy[pick].cpu(), ws, w.cpu(), wr, ds[pick].cpu())
+    rounded(dx[pick], wx, 2 * NORM * mx)
+    n = s.double() * rstd.double()[:, None]
+    near(dw, (dy.double() * n).sum(0).cpu(), (rows + 40) * U * (dy.double() * n).abs().sum(0).cpu())
+    need = int(_lib.load().dssm_rms_norm_bwd_ws_bytes(rows, cols))
+    ws_ = torch.empty(need, dtype=torch.uint8, device=device)
+    for turn in range(2):
+        a, b, c, d = x.clone(), res.clone(), dy.clone(), ds.clone()
+        over, back = (a, c) if turn else (b, d)
+        y2, r2, w2 = torch.empty_like(y), torch.empty_like(rstd), torch.empty_like(dw)
+        seqops._call(0, "dssm_rms_norm", a.data_ptr(), cols, b.data_ptr(), cols, w.data_ptr(), rows, cols, code, 1e-6,
+                     y2.data_ptr(), cols, over.data_ptr(), cols, r2.data_ptr())
+        assert torch.equal(y2, y) and torch.equal(over, s) and torch.equal(r2, rstd)
+        seqops._call(0, "dssm_rms_norm_bwd", c.data_ptr(), cols, s.data_ptr(), cols, w.data_ptr(), rstd.data_ptr(),
+                     d.data_ptr(), cols, rows, cols, code, back.data_ptr(), cols, w2.data_ptr(), ws_.data_ptr(), need)
+        assert torch.equal(back, dx) and torch.equal(w2, dw)
 
 
 def test_norm_gradient_against_differences(device):
