@@ -11,12 +11,12 @@
 // spread over as many workgroups as any other half.
 //
 // The sort is a least-significant-digit radix sort of (token, position) pairs, digits of at most 10 bits;
-// a workgroup ranks a tile of 4096 pairs by wave ballots.  The rows of zeros that untouched tokens need
+// a workgroup ranks a tile of 1024 or 4096 pairs by wave ballots.  The rows of zeros that untouched tokens need
 // are written by extra workgroups of the sort's launches, whose own work is latency.
 //
 // Measured, 196608 tokens of 128 columns over 21128 words (log-uniform; 62 MB that must move, 12.7 us at the
 // rate of a large copy): lookup fp32 -> bf16 14.3 us, 4.3 TB/s; gradient of bf16 rows 49 us in six launches:
-// per digit count 3.2 and place 8.8 us (loads, tile sums and ranks one behind the other: latency), spans 20
+// per digit count 3.2 and place 8.8 us (loads, tile sums and ranks one behind the other: latency), spans 19
 // (50 MB of gathered rows, every workgroup resident at once: the rows' own time and two latencies), join 7.
 #include <hip/hip_runtime.h>
 
@@ -349,9 +349,9 @@ template <typename T, int V>
 __global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pairs, int64_t n, unsigned words,
                                                     const T* __restrict__ dy, int64_t lddy, int E, float scale,
                                                     float* __restrict__ dtable, float* __restrict__ part, int lg) {
-  __shared__ float came[V * 256], goes[V * 256];
-  __shared__ unsigned char flags[256];
-  enum { kOut = 1, kOne = 2 };  // the last run goes on into the next stretch; there is one run
+  constexpr int kAt = V == 1 ? 8 : 2;  // pieces of a run that are read at once
+  __shared__ __attribute__((aligned(16))) float came[256 * V], goes[256 * V];
+  __shared__ unsigned long long through[4];  // bits of the threads whose stretch is one run that goes on into the next
   const int G = 1 << lg, groups = 256 >> lg, g = threadIdx.x >> lg, lane = threadIdx.x & (G - 1);
   const int64_t i0 = ((int64_t)blockIdx.x * groups + g) * kStretch, i1 = min(i0 + kStretch, n);
   const unsigned none = 0xffffffffu;
@@ -363,7 +363,9 @@ __global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pa
 #pragma unroll
   for (int j = 1; j < kStretch; ++j) last = k[j].x != none ? k[j].x : last;
   const bool live = i0 < n, in = live && k[0].x == prev, out = live && last == next;
-  if (lane == 0) flags[g] = (out ? kOut : 0) | (k[0].x == last ? kOne : 0);
+  const bool one = k[0].x == last;  // the stretch is one run
+  const unsigned long long pass = __ballot(one && out);
+  if ((threadIdx.x & 63) == 0) through[threadIdx.x >> 6] = pass;
   for (int c0 = 0; c0 < E; c0 += G * V) {
     const int c = c0 + lane * V;
     const bool mine = c < E;
@@ -386,7 +388,7 @@ __global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pa
           if (incoming || outgoing) {
             float* to = incoming ? came : goes;
 #pragma unroll
-            for (int q = 0; q < V; ++q) to[q * 256 + threadIdx.x] = acc[q];
+            for (int q = 0; q < V; ++q) to[threadIdx.x * V + q] = acc[q];
           } else {
             Pack<float, V> y;
 #pragma unroll
@@ -401,7 +403,7 @@ __global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pa
     }
     __syncthreads();
     // Who joins a run's pieces: the group where it starts, or group 0 for the one that came into the span.
-    const bool starts = out && !(in && (flags[g] & kOne)) && last < words;
+    const bool starts = out && !(in && one) && last < words;
     const bool enters = g == 0 && in && k[0].x < words;
 #pragma unroll
     for (int role = 0; role < 2; ++role) {
@@ -409,13 +411,31 @@ __global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pa
       const float* from = role ? goes : came;
       float sum[V];
 #pragma unroll
-      for (int q = 0; q < V; ++q) sum[q] = from[q * 256 + threadIdx.x];
-      bool on = role || ((flags[0] & kOne) && out);  // the run reaches the next stretch
-      int j = g + 1;
-      for (; on && j < groups; ++j) {
+      for (int q = 0; q < V; ++q) sum[q] = from[threadIdx.x * V + q];
+      bool on = role || (one && out);  // the run reaches the next stretch
+      if (on) {
+        // the run's last piece here: that of the first group behind this one which it does not pass through
+        int e = groups;
+        const int t0 = (g + 1) << lg;  // (thread 256 is none: the last group's run leaves the span)
+        for (int w = t0 >> 6; w < 4 && e == groups; ++w) {
+          const unsigned long long stop = ~through[w] & (w == t0 >> 6 ? ~0ull << (t0 & 63) : ~0ull);
+          if (stop) e = (w * 64 + __ffsll(stop) - 1) >> lg;
+        }
+        on = e == groups;
+        const int n1 = min(e + 1, groups);
+        // in order, several pieces' reads at once (one by one, each behind its own flag, took this launch 17 us
+        // where it takes 12: 8955 x 24 fp16 over 56 words; more at once take registers that waves need)
+        for (int j = g + 1; j < n1; j += kAt) {
+          float x[kAt][V];
 #pragma unroll
-        for (int q = 0; q < V; ++q) sum[q] += came[q * 256 + (j << lg) + lane];
-        on = (flags[j] & kOne) && (flags[j] & kOut);
+          for (int u = 0; u < kAt; ++u)
+#pragma unroll
+            for (int q = 0; q < V; ++q) x[u][q] = j + u < n1 ? came[((((j + u) << lg) + lane) & 255) * V + q] : 0.f;
+#pragma unroll
+          for (int u = 0; u < kAt; ++u)
+#pragma unroll
+            for (int q = 0; q < V; ++q) sum[q] += x[u][q];
+        }
       }
       if (role && !on) {
         Pack<float, V> y;
