@@ -12,12 +12,13 @@
 //   g_t = dh_t + u_{t+1} g_{t+1},  dcand_t = (1 - u_t) g_t,  dgate_t = g_t (h_{t-1} - cand_t) u_t (1 - u_t),
 // with gamma = u g as the value that crosses from step to step (gamma -> P gamma + Q over a stretch).
 //
-// Layout: a lane owns 4 bytes of neighbouring channels of one row, a wave a piece of kPiece steps whose
-// loads are all in flight at once.  With few channels NW waves take NW consecutive pieces: each reduces
-// its piece to (A, B), they meet in LDS once, and each replays its piece from registers behind its true
-// state, so the inputs are read once.  With very few channels the time axis is also cut into segments of
-// several workgroups: one launch reduces the segments, the next folds the earlier segments' (A, B) into
-// its own start; there the inputs are read twice.
+// Layout: a lane owns up to 4 bytes of neighbouring channels of one row (the last lane of an odd number of 16-bit
+// channels shares one with its neighbour, and both store the same: 8 x 4365 x 629 bf16 59 + 89 us, 79 + 111 with
+// a channel a lane), a wave a piece of kPiece steps whose loads are all in flight at once.  With few channels NW
+// waves take NW consecutive pieces: each reduces its piece to (A, B), they meet in LDS once, and each replays its
+// piece from registers behind its true state, so the inputs are read once.  With very few channels the time axis
+// is also cut into segments of several workgroups: one launch reduces the segments, the next folds the earlier
+// segments' (A, B) into its own start; there the inputs are read twice.
 //
 // The forward keeps the fp32 state in front of every piece (half a byte per element); the
 // backward walks a piece forward from it in registers and so needs neither h nor a forward scan.  States,
@@ -89,7 +90,7 @@ __device__ __forceinline__ Unit<V> unit_of(const RecurArgs& a, int64_t u) {
   t.in = u < a.R * a.upr;
   if (!t.in) u = a.R * a.upr - 1;
   t.r = u / a.upr;
-  t.c = (int)(u - t.r * a.upr) * V;
+  t.c = min((int)(u - t.r * a.upr) * V, a.H - V);
   t.ch = t.r * a.H + t.c;
   int len = a.T;
   if (a.lens) len = min(max(a.lens[t.r], 0), a.T);
@@ -479,20 +480,23 @@ __global__ __launch_bounds__(256) void k_recur_step(const T* __restrict__ gate, 
   stv<T, V>(h + r * hr + c, o);
 }
 
-// How the work is cut.  `waves`: waves of 64 lanes that the channels alone give.  From 1024 on (one for each SIMD)
-// a wave walks its row alone; below it, four or eight share the time of a workgroup's channels, and where even
-// that leaves fewer than 2048 waves, time is cut into segments until there are 4096 (2 x 65537 x 512: 140 us;
-// 181 with 2048, 154 with 8192), of two rounds of pieces at least.  Up to four rounds stay one launch, whose rounds cost
-// less than a second launch's start (8 x 128 bf16: 133 steps 8.4 and 11.6 us, 11.8 and 15.4 cut; 256 steps 10.4 and
-// 16.4, 12.0 and 15.6 cut; 512 steps 18.4 and 29.7, 12.1 and 15.7 cut).
+// How the work is cut.  16-bit channels go two a lane (64 x 100 x 512 bf16 16.3 and 22.3 us, 18.3 and 24.1 with one;
+// 64 x 256 x 8192 268 and 419, 297 and 466), but one where the work is small and a lane's own time counts (8 x 128 x
+// 133 bf16 7.0 and 9.5 us, 8.4 and 11.6 with two; 16 x 256 x 512 11.2 and 14.6, 12.7 and 17.0).
+// `waves`: waves of 64 lanes that the channels alone give.  From 1024 on (one for each SIMD) a wave walks its row
+// alone; below it, four or eight share the time of a workgroup's channels, and where even that leaves fewer than 2048
+// waves, time is cut into segments until there are 4096 (2 x 65537 x 512: 140 us; 181 with 2048, 154 with 8192), of
+// two rounds of pieces at least.  Up to four rounds stay one launch, whose rounds cost less than a second launch's
+// start (8 x 128 bf16, two channels a lane: 133 steps 8.4 and 11.6 us, 11.8 and 15.4 cut; 256 steps 10.4 and 16.4,
+// 12.0 and 15.6 cut; 512 steps 18.4 and 29.7, 12.1 and 15.7 cut).
 struct Cut {
   int V, NW, S, L;
 };
 Cut cut_of(int64_t R, int T, int H, int dtype) {
   Cut c{};
-  const int wide = dtype == DSSM_F32 ? 1 : 2;
-  c.V = H % wide ? 1 : wide;
-  const int64_t waves = (R * (H / c.V) + 63) / 64;
+  const bool small = R * H < 64 * 1024 && (double)R * H * T < 3e6;
+  c.V = dtype == DSSM_F32 || H < 2 || small ? 1 : 2;
+  const int64_t waves = (R * ((H + c.V - 1) / c.V) + 63) / 64;
   const int pieces = (T + kPiece - 1) / kPiece;
   c.NW = 1;
   c.S = 1;
@@ -534,7 +538,7 @@ void launch(const RecurArgs& a, const Cut& c, hipStream_t s) {
 template <bool FWD>
 int run(RecurArgs& a, int dtype, void* stream) {
   const Cut c = cut_of(a.R, a.T, a.H, dtype);
-  a.upr = a.H / c.V;
+  a.upr = (a.H + c.V - 1) / c.V;
   a.S = c.S;
   a.L = c.L;
   // a wave's 64 units lie in at most 64 / upr + 2 rows: do all their offsets fit 32 bits?

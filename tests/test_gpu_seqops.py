@@ -161,7 +161,8 @@ def check_recurrence(device, gate, cand, lens, h0, reverse, g, grad=True):
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("R,T,H,dtype", [(1, 1, 1, F32), (3, 1, 5, BF), (2, 16, 6, F16), (5, 17, 33, BF), (4, 40, 64, BF),
                                          (3, 63, 10, F32), (2, 129, 130, F16), (600, 33, 128, BF), (2100, 18, 64, F32),
-                                         (1050, 20, 65, F16), (2, 256, 6, BF), (2, 257, 6, F32), (3, 300, 7, BF), (1, 1029, 3, F32), (2, 2500, 20, BF)])
+                                         (1050, 20, 65, F16), (2, 256, 6, BF), (2, 257, 6, F32), (3, 300, 7, BF),
+                                         (1, 1029, 3, F32), (2, 2500, 20, BF), (20, 2500, 63, BF), (14, 3400, 66, F16)])
 def test_recurrence(device, R, T, H, dtype, reverse):
     gate, cand, lens, h0, g = inputs(R, T, H, dtype, R + T + H)
     check_recurrence(device, gate, cand, lens, h0, reverse, g)
@@ -264,6 +265,25 @@ def test_recurrence_strides(device, dtype):
     h, _ = api.linear_recurrence(args[0][:1].expand(R, T, H), args[1])
     h2, _ = api.linear_recurrence(args[0][:1].repeat(R, 1, 1), args[1])
     assert torch.equal(h, h2)
+
+
+def test_recurrence_strides_of_long_rows(device):
+    """An odd number of 16-bit channels, two a lane, in segments of time; rows that start anywhere, and rows so far
+    apart that a wave's offsets pass 32 bits."""
+    R, T, H, far = 2, 24011, 65, 340_000_000
+    g = torch.Generator(device).manual_seed(3)
+    args = [torch.randn(R, T, H, generator=g, device=device).to(BF) for _ in range(3)]
+    want = api.linear_recurrence(args[0], args[1], save=True)
+    wgrad = api.linear_recurrence_grad(args[0], args[1], want[2], args[2])
+    odd = torch.zeros(R, T, 3 * H + 2, dtype=BF, device=device)
+    near_ = [odd[..., k * H + 1:(k + 1) * H + 1] for k in range(3)]
+    away = [torch.zeros(far * (R - 1) + T * H, dtype=BF, device=device).as_strided((R, T, H), (far, H, 1)) for _ in range(3)]
+    for xs in (near_, away):
+        for x, y in zip(xs, args):
+            x.copy_(y)
+        got = api.linear_recurrence(xs[0], xs[1], save=True)
+        for a, b in zip(got + api.linear_recurrence_grad(xs[0], xs[1], got[2], xs[2]), want + wgrad):
+            assert torch.equal(a, b)
 
 
 def test_recurrence_empty(device):
