@@ -17,7 +17,7 @@
 // Measured, 196608 tokens of 128 columns over 21128 words (log-uniform; 62 MB that must move, 12.7 us at the
 // rate of a large copy): lookup fp32 -> bf16 14.3 us, 4.3 TB/s; gradient of bf16 rows 49 us in six launches:
 // per digit count 3.2 and place 8.8 us (loads, tile sums and ranks one behind the other: latency), spans 19
-// (50 MB of gathered rows, every workgroup resident at once: the rows' own time and two latencies), join 7.
+// (50 MB of gathered rows, every workgroup resident at once: the rows' own time and two latencies), join 6.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -511,12 +511,13 @@ __global__ __launch_bounds__(256) void k_grad_join(const uint2* __restrict__ pai
     const int64_t h = longs[j];
     const unsigned tok = pairs[(h + 1) * S].x;
     // the run's last span: the last one whose first entry is still this token.  The list is sorted, so of 256
-    // probes at equal distances a first few are this token's, and the last of those bounds the next round.
+    // probes at equal distances a first few are this token's, and the last of those bounds the next round; the
+    // first round looks at the next 256 spans, where nearly every run ends.
     int64_t lo = h + 1, hi = spans - 1;
-    while (lo < hi) {
-      const int64_t gap = (hi - lo + 255) / 256, at = lo + (threadIdx.x + 1) * gap;
+    for (bool first = true; lo < hi; first = false) {
+      const int64_t gap = first ? 1 : (hi - lo + 255) / 256, at = lo + (threadIdx.x + 1) * gap;
       const int hit = __syncthreads_count(at <= hi && pairs[at * S].x == tok);
-      hi = min(hi, lo + (hit + 1) * gap - 1);
+      if (hit < 256 || !first) hi = min(hi, lo + (hit + 1) * gap - 1);
       lo += hit * gap;
     }
     const int64_t cnt = lo - h, per = (cnt + groups - 1) / groups;

@@ -97,6 +97,16 @@ def test_lookup_grad_patterns(device, n, E, kind):
     check_grad(device, dy, ids, V)
 
 
+def test_lookup_grad_runs_of_about_256_spans(device):
+    """Runs whose last span is found by one look at the next 256, just so, and by further ones; rows of 130 columns
+    have spans of 32 entries."""
+    g = gen(21)
+    ids = torch.cat([torch.full((32 * k + d,), i) for i, (k, d) in enumerate(
+        [(255, 0), (256, 0), (257, 31), (258, 1), (3, 5), (254, 30), (513, 2), (9, 0), (256, 31), (600, 7)])])
+    check_grad(device, torch.randn(len(ids), 130, generator=g), ids, 12)
+    check_grad(device, torch.randn(len(ids), 130, generator=g), ids[torch.randperm(len(ids), generator=g)], 12)
+
+
 def test_lookup_grad_repeats_bit_for_bit_and_strides(device):
     g = gen(8)
     ids = (torch.rand(30000, generator=g) ** 4 * 500).long().to(device)
