@@ -69,7 +69,8 @@ __device__ __forceinline__ void store4(const Gemm8Args& g, int m, int n, f32x4 v
 }
 
 // ---- tiles -------------------------------------------------------------------------------------
-// A workgroup of WM x WN waves computes (WM MI 32) x (WN NI 32) outputs with v_mfma_scale_f32_32x32x64.
+// A group of WM x WN waves computes (WM MI 32) x (WN NI 32) outputs with v_mfma_scale_f32_32x32x64; SK groups of a
+// workgroup take a share of K each, in LDS of their own, and meet at the end.
 //
 // Both operands go from memory straight to LDS, 16 bytes a lane, a block of 128 columns at a time into one of D
 // buffers; whole 128-byte lines, because the two halves of a line that are asked for apart meet as one pending
@@ -77,8 +78,8 @@ __device__ __forceinline__ void store4(const Gemm8Args& g, int m, int n, f32x4 v
 // multiplies fragments that are in registers already while it reads the next round's: when a block's second
 // round begins, nobody needs its buffer any more, and the block D further on is asked for, 2 (D - 1) rounds of
 // products before its first fragment is read.  D is 2 for the large tiles (256 x 256: 128 KB of LDS, 2048 cycles
-// of the matrix units ahead); 64 x 64, which runs where there are few tiles and the memory's latency is all
-// there is to a block, takes 4.
+// of the matrix units ahead); 64 x 64 and 32 x 32, which run where there are few tiles and the memory's latency is
+// all there is to a block, take 4.
 //
 // Measured, 8192 x 4096 x 8192: 226 us, 2.4 PFLOP/s, 93 % of the library's rate for one scale a tensor (2.56); the
 // matrix units are busy 62 % of the time at 1.85 GHz, to which their power brings the clock down.  Without the loads
@@ -89,21 +90,27 @@ __device__ __forceinline__ void store4(const Gemm8Args& g, int m, int n, f32x4 v
 // conflict counter, which reads zero); of these rows no two of the same parity have the same r >> 1 & 7, so
 // they cover all 64 banks.  The direct load writes LDS in lane order, so the permutation is applied to the
 // address that each lane loads from.
-template <int WM, int WN, int MI, int NI, int D, typename O>
-__global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Gemm8Args g) {
-  constexpr int BM = WM * MI * 32, BN = WN * NI * 32, NW = WM * WN, kLoads = (BM + BN) / 8 / NW;
+template <int WM, int WN, int MI, int NI, int D, int SK, typename O>
+__global__ __launch_bounds__(WM * WN * SK * 64, WM * WN * SK == 8 ? 2 : 1) void k_gemm8(Gemm8Args g) {
+  constexpr int BM = WM * MI * 32, BN = WN * NI * 32, NW = WM * WN, kLoads = (BM + BN) / 8 / NW;  // (of one group)
   static_assert(kLoads * 8 * NW == BM + BN && BM % 8 == 0, "every wave loads the same number of 8-row stripes");
   // Scales.  The large tiles keep a word a row, four blocks' bytes, which a thread loads for a row at a time.  The
-  // small one sends a byte a row and block the operands' way (the load widens it to a word): no wait of its own,
+  // small ones send a byte a row and block the operands' way (the load widens it to a word): no wait of its own,
   // for more work in the vector cache, which they leave idle.
   constexpr bool kWords = D == 2;
   constexpr int kScaleRows = (BM + BN) / (NW * 64) ? (BM + BN) / (NW * 64) : 1;  // a thread's
-  static_assert(BM % 64 == 0 && (kScaleRows * NW * 64 == BM + BN || !kWords), "a row's scales are loaded by one thread");
+  static_assert((BM + BN) % 64 == 0 && (kScaleRows * NW * 64 == BM + BN || !kWords), "a row's scales are loaded by one thread");
   // D blocks, then the scales.  One object: of two the compiler knows that they are two, tells the direct loads
   // apart by that, and puts a wait for all of them in front of every read.
-  constexpr int kBuf = (BM + BN) * kBlk, kScale = (BM + BN) * 4;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[D * kBuf + D * kScale];
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % WM, wn = wv / WM;
+  constexpr int kBuf = (BM + BN) * kBlk, kScale = (BM + BN) * 4, kGroup = D * kBuf + D * kScale;
+  static_assert(SK == 1 || !kWords, "the words are put by the whole workgroup");
+  __shared__ __attribute__((aligned(16))) unsigned char shared[SK * kGroup];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = SK == 1 ? 0 : wave / NW, wv = SK == 1 ? wave : wave % NW, wm = wv % WM, wn = wv / WM;
+  const int thread = SK == 1 ? threadIdx.x : threadIdx.x % (NW * 64);
+  unsigned char* const lds = shared + grp * kGroup;
+  // this group's blocks: `per` from k0 on, of which the first `own` are its own (the walk is as long for every group)
+  const int per = SK == 1 ? g.KB : (g.KB + SK - 1) / SK, k0 = grp * per, own = g.KB - k0;
   const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN;
   // neighbouring tiles to one XCD, in bands of 8 tile rows whose operands its L2 keeps
   int t = xcd_tile(blockIdx.x, tm * tn);
@@ -126,7 +133,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
   }
   // (behind the last block the last one is loaded again, into a half that serves no more: no branch)
   auto load = [&](int kb, int from, int to) {
-    const unsigned at = (unsigned)min(kb, g.KB - 1) * kBlk;
+    const unsigned at = (unsigned)min(k0 + kb, g.KB - 1) * kBlk;
 #pragma unroll
     for (int i = from; i < to; ++i)
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(base[i] + at + off[i]),
@@ -139,7 +146,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
   unsigned sword[kScaleRows];
 #pragma unroll
   for (int i = 0; i < kScaleRows; ++i) {
-    const int r = i * NW * 64 + threadIdx.x;
+    const int r = i * NW * 64 + thread;
     srow[i] = r < BM ? g.ea + (int64_t)min(m0 + r, g.M - 1) * g.KB : g.ew + (int64_t)min(n0 + r - BM, g.N - 1) * g.KB;
     if (kWords) sword[i] = scale4(srow[i], 0, g.KB);
   }
@@ -151,14 +158,14 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
     const int behind = g.KB >= 4 ? max(0, kb + 4 - g.KB) : 0;
 #pragma unroll
     for (int i = 0; i < kScaleRows; ++i)
-      *reinterpret_cast<unsigned*>(&lds[D * kBuf + (kb >> 2 & 1) * kScale + (i * NW * 64 + threadIdx.x) * 4]) =
+      *reinterpret_cast<unsigned*>(&lds[D * kBuf + (kb >> 2 & 1) * kScale + (i * NW * 64 + thread) * 4]) =
           sword[i] >> (8 * behind);
   };
   auto load_scales = [&](int kb) {
 #pragma unroll
     for (int i = 0; i < kScaleRows; ++i)
       if ((i * NW + wv) * 64 < BM + BN)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(srow[i] + min(kb, g.KB - 1)),
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)(srow[i] + min(k0 + kb, g.KB - 1)),
                                          (__attribute__((address_space(3))) unsigned*)&lds[D * kBuf + (kb & (D - 1)) * kScale +
                                                                                             (i * NW + wv) * 256],
                                          1, 0, 0);
@@ -182,6 +189,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
   };
   i32x8 fa[MI], w0[NI], w1[NI];
   int sa[MI], sw[NI], na[MI], nw[NI];
+  int mine = -1;  // 0: the block is behind this group's last and counts as zeros (a NaN in it is in the result anyway)
   auto fetch_scales = [&](int kb) {
     const unsigned char* at = lds + D * kBuf + (kWords ? (kb >> 2 & 1) * kScale + (kb & 3) : (kb & (D - 1)) * kScale);
 #pragma unroll
@@ -198,6 +206,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
+      if constexpr (SK > 1) fa[i] &= mine;
 #pragma unroll
       for (int j = 0; j < NI; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[j], fa[i], acc[i][j], 0, 0, 0, sw[j], 0, sa[i]);
@@ -226,7 +235,8 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
 #pragma unroll
   for (int i = 0; i < MI; ++i) fa[i] = frag(0, 0, ra + i * 32 * kBlk);
   fetch_scales(0);
-  for (int kb = 0; kb < g.KB; ++kb) {
+  for (int kb = 0; kb < per; ++kb) {
+    if constexpr (SK > 1) mine = kb < own ? -1 : 0;
 #pragma unroll
     for (int i = 0; i < MI; ++i) sa[i] = na[i];
 #pragma unroll
@@ -253,12 +263,43 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
   // a row of the result.  The tile is put together in LDS, so that its rows leave in whole lines: stored from
   // the registers they cost the L2 twelve times the requests.  Piece c (16 bytes) of row r lies at c ^ (r % kPieces).
   asm volatile("s_barrier" ::: "memory");  // all waves are past their last reads of the operands
+  constexpr int kTile = BM * BN * 2;
+  if constexpr (SK > 1) {  // the groups' sums, in their order
+    static_assert(kTile + (SK - 1) * BM * BN * 4 <= SK * kGroup, "they fit behind the tile");
+    f32x4* const sums = reinterpret_cast<f32x4*>(shared + kTile);
+    if (grp) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            sums[((((grp - 1) * NW + wv) * MI * NI + i * NI + j) * 4 + q) * 64 + lane] =
+                f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    }
+    __syncthreads();
+    if (!grp) {
+#pragma unroll
+      for (int k = 0; k < SK - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const f32x4 v = sums[(((k * NW + wv) * MI * NI + i * NI + j) * 4 + q) * 64 + lane];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
+            }
+    }
+  }
   constexpr int kPieces = BN / 8;
-  static_assert(BM * BN * 2 <= D * kBuf && (kPieces & (kPieces - 1)) == 0, "the tile fits where the operands were");
+  static_assert(kTile <= D * kBuf && (kPieces & (kPieces - 1)) == 0, "the tile fits where the operands were");
 #pragma unroll
   for (int j = 0; j < NI; ++j)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
+      if (grp) break;
       const int n = (wn * NI + j) * 32 + 8 * q + 4 * fg;
       float add[4];
 #pragma unroll
@@ -269,15 +310,15 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 1) void k_gemm8(Ge
         Pack<O, 4> y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) y.v[e] = st1<O>(acc[i][j][4 * q + e] + add[e]);
-        *reinterpret_cast<uint2*>(&lds[r * BN * 2 + (((n >> 3) ^ (r & (kPieces - 1))) << 4) + (n & 4) * 2]) =
+        *reinterpret_cast<uint2*>(&shared[r * BN * 2 + (((n >> 3) ^ (r & (kPieces - 1))) << 4) + (n & 4) * 2]) =
             __builtin_bit_cast(uint2, y);
       }
     }
   __syncthreads();
-  for (int u = threadIdx.x; u < BM * kPieces; u += NW * 64) {
+  for (int u = threadIdx.x; u < BM * kPieces; u += NW * SK * 64) {
     const int r = u / kPieces, c = u % kPieces, n = n0 + c * 8;
     if (m0 + r >= g.M || n >= g.N) continue;
-    const uint4 y = *reinterpret_cast<const uint4*>(&lds[r * BN * 2 + ((c ^ (r & (kPieces - 1))) << 4)]);
+    const uint4 y = *reinterpret_cast<const uint4*>(&shared[r * BN * 2 + ((c ^ (r & (kPieces - 1))) << 4)]);
     const Pack<O, 8> p = __builtin_bit_cast(Pack<O, 8>, y);
     O* to = (O*)g.out + (int64_t)(m0 + r) * g.ldo + n;
     if (n + 8 <= g.N) {
@@ -368,20 +409,27 @@ int run_gemm8(const Gemm8Args& g, hipStream_t s) {
   const auto tiles = [&](int b) { return (int64_t)((g.M + b - 1) / b) * ((g.N + b - 1) / b); };
   if (tiles(64) > 0x7fffffff) return dssm::report_error(DSSM_E_UNSUPPORTED, "blocks8_matmul: too many outputs");
   const int tile = tile_of(tiles(64), tiles(128), tiles(256));
-  // Rows against rows where a is short, or where all the outputs are few: the waves of a workgroup share K (7 x 4096
-  // x 4096: 6.1 us against 11.2 in 64 x 64 tiles, 32 x 256 x 8192 10.0 against 18.1, 100 x 300 x 200 2.9 against
-  // 4.3); 32 rows at a time for 17 to 32 of them (32 x 4096 x 4096: 8.9 us, 10.7 sixteen at a time, 11.4 in tiles).
+  // Rows against rows where that takes a workgroup a compute unit at most: the waves of a workgroup share K (7 x 4096 x
+  // 4096: 5.9 us against 8.5 in 32 x 32 tiles, 32 x 256 x 8192 10.0 against 11.6, 100 x 300 x 200 2.9 against 4.3);
+  // 32 rows at a time for 17 to 32 of them (32 x 4096 x 4096: 8.8 us, 10.7 sixteen at a time, 9.1 in tiles).  With more
+  // workgroups, each of which reads its rows of a again, tiles are faster (32 x 8192 x 1024 5.6 us against 8.4, 16 x
+  // 12288 x 4096 12.3 against 14.6).
   const int64_t n16 = (g.N + 15) / 16, m16 = (g.M + 15) / 16;
-  if (g.M <= 16 || n16 * m16 <= 256) {
+  if (n16 * m16 <= 256) {
     hipLaunchKernelGGL((k_gemm8_rows<1, O>), dim3((unsigned)n16, (unsigned)m16), dim3(512), 0, s, g);
-  } else if (g.M <= 32) {
+  } else if (g.M <= 32 && n16 <= 256) {
     hipLaunchKernelGGL((k_gemm8_rows<2, O>), dim3((unsigned)n16, 1), dim3(512), 0, s, g);
+  } else if (tiles(32) <= 256 && g.KB >= 8) {
+    // A tile's time is what its compute unit can load: 32 x 32 while these find a unit each, and two blocks for each
+    // of the four groups of waves that share K (64 x 4096 x 4096 9.3 us, 11.8 in 64 x 64 tiles; 256 x 1024 x 8192
+    // 13.1 and 19.6; of two rounds 12.0 and 12.1; 64 x 4096 x 384 4.6 and 4.3)
+    hipLaunchKernelGGL((k_gemm8<1, 1, 1, 1, 4, 4, O>), dim3((unsigned)tiles(32)), dim3(256), 0, s, g);
   } else if (tile == 64) {
-    hipLaunchKernelGGL((k_gemm8<2, 2, 1, 1, 4, O>), dim3((unsigned)tiles(64)), dim3(256), 0, s, g);
+    hipLaunchKernelGGL((k_gemm8<2, 2, 1, 1, 4, 1, O>), dim3((unsigned)tiles(64)), dim3(256), 0, s, g);
   } else if (tile == 128) {
-    hipLaunchKernelGGL((k_gemm8<2, 2, 2, 2, 2, O>), dim3((unsigned)tiles(128)), dim3(256), 0, s, g);
+    hipLaunchKernelGGL((k_gemm8<2, 2, 2, 2, 2, 1, O>), dim3((unsigned)tiles(128)), dim3(256), 0, s, g);
   } else {
-    hipLaunchKernelGGL((k_gemm8<2, 4, 4, 2, 2, O>), dim3((unsigned)tiles(256)), dim3(512), 0, s, g);
+    hipLaunchKernelGGL((k_gemm8<2, 4, 4, 2, 2, 1, O>), dim3((unsigned)tiles(256)), dim3(512), 0, s, g);
   }
   return seq_status(hipGetLastError());
 }

@@ -593,7 +593,8 @@ def product(a, w, bias, K):
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 300, 128), (7, 17, 129), (16, 40, 1000), (17, 64, 2000), (33, 130, 257),
                                    (65, 300, 513), (64, 16, 4500), (200, 77, 640), (1100, 1030, 300), (257, 4100, 400),
                                    (3000, 3001, 130), (1500, 1500, 100), (1500, 1500, 1300), (200, 500, 3000),
-                                   (100, 300, 200), (3000, 3001, 1100)])
+                                   (100, 300, 200), (3000, 3001, 1100), (40, 4000, 1030), (250, 1000, 1700),
+                                   (100, 1500, 2100), (9, 4200, 1300), (20, 4200, 200), (180, 700, 1024)])
 def test_product(device, M, N, K, out):
     g = gen(M + N + K)
     a = api.quantize_blocks8((torch.randn(M, K, generator=g) * torch.exp(torch.randn(M, 1, generator=g))).to(device))
@@ -623,6 +624,23 @@ def test_product_scales_and_rows_are_apart(device):
         assert bad[M // 2].all() and bad[:, N - 1].all() and bad.sum() == M + N - 1
         want, tol = product(a, w, None, K)
         rounded(got.cpu()[~bad], want[~bad], tol[~bad])
+
+
+def test_product_shares_of_k(device):
+    """Four groups of waves share nine blocks: the shares that are not there add nothing, not even the NaN that the
+    last block holds, and that one's scale."""
+    M, N, K = 200, 500, 1100
+    g = gen(77)
+    x, y = torch.randn(M, K, generator=g), torch.randn(N, K, generator=g)
+    x[3, K - 1], y[7, K - 2], x[150, 0] = float("nan"), float("inf"), float("nan")
+    a, w = api.quantize_blocks8(x.to(device)), api.quantize_blocks8(y.to(device))
+    a.scale.view(torch.uint8)[9, 8] = 255
+    w.scale.view(torch.uint8)[11, 8] = 255
+    bad = torch.isnan(api.blocks8_matmul(a, w).cpu())
+    want = torch.zeros(M, N, dtype=torch.bool)
+    want[[3, 9, 150]] = True
+    want[:, [7, 11]] = True
+    assert torch.equal(bad, want)
 
 
 def test_product_empty(device):
