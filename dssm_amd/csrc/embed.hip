@@ -319,7 +319,7 @@ __global__ __launch_bounds__(1024) void k_sort_place(const I* __restrict__ ids, 
     *reinterpret_cast<uint4*>(sum + 4096 + q * bins + d4 * 4) = b4;
     __syncthreads();
     if ((int)threadIdx.x < bins)
-      for (int i = 0; i < share; ++i) {
+      for (int i = 0; i < min(share, tiles); ++i) {
         all += sum[i * bins + threadIdx.x];
         before += sum[4096 + i * bins + threadIdx.x];
       }
@@ -345,11 +345,11 @@ __global__ __launch_bounds__(1024) void k_sort_place(const I* __restrict__ ids, 
 // piece that starts in s and goes on) for k_grad_join.  A piece that fills its span counts as incoming.
 constexpr int kStretch = 8;
 
-template <typename T, int V>
+template <typename T, int V, bool TREE>
 __global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pairs, int64_t n, unsigned words,
                                                     const T* __restrict__ dy, int64_t lddy, int E, float scale,
                                                     float* __restrict__ dtable, float* __restrict__ part, int lg) {
-  constexpr int kAt = V == 1 ? 8 : 2;  // pieces of a run that are read at once
+  constexpr int kAt = TREE ? 1 : V == 1 ? 8 : 2;  // pieces of a run that are read at once
   __shared__ __attribute__((aligned(16))) float came[256 * V], goes[256 * V];
   __shared__ unsigned long long through[4];  // bits of the threads whose stretch is one run that goes on into the next
   const int G = 1 << lg, groups = 256 >> lg, g = threadIdx.x >> lg, lane = threadIdx.x & (G - 1);
@@ -366,6 +366,17 @@ __global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pa
   const bool one = k[0].x == last;  // the stretch is one run
   const unsigned long long pass = __ballot(one && out);
   if ((threadIdx.x & 63) == 0) through[threadIdx.x >> 6] = pass;
+  // the last stretch of the run that comes into stretch `from`: the first from there on that is not passed through
+  // (groups: the run goes on behind the span)
+  auto first_stop = [&](int from) {
+    int e = groups;
+    const int t0 = from << lg;
+    for (int w = t0 >> 6; w < 4 && e == groups; ++w) {
+      const unsigned long long stop = ~through[w] & (w == t0 >> 6 ? ~0ull << (t0 & 63) : ~0ull);
+      if (stop) e = (w * 64 + __ffsll(stop) - 1) >> lg;
+    }
+    return e;
+  };
   for (int c0 = 0; c0 < E; c0 += G * V) {
     const int c = c0 + lane * V;
     const bool mine = c < E;
@@ -402,6 +413,26 @@ __global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pa
       }
     }
     __syncthreads();
+    if constexpr (TREE) {
+      // came[g] becomes the sum of a run's pieces from stretch g to its last one here, by doubling (but for g = 0).
+      // What no run has brought is not used.
+      const int end = first_stop(g);
+      for (int d = 1; d < groups; d <<= 1) {
+        const bool more = g && g + d <= min(end, groups - 1);
+        if (!__syncthreads_or(more)) break;
+        float x[V];
+        if (more && mine) {
+#pragma unroll
+          for (int q = 0; q < V; ++q) x[q] = came[threadIdx.x * V + q] + came[(threadIdx.x + (d << lg)) * V + q];
+        }
+        __syncthreads();
+        if (more && mine) {
+#pragma unroll
+          for (int q = 0; q < V; ++q) came[threadIdx.x * V + q] = x[q];
+        }
+      }
+      __syncthreads();
+    }
     // Who joins a run's pieces: the group where it starts, or group 0 for the one that came into the span.
     const bool starts = out && !(in && one) && last < words;
     const bool enters = g == 0 && in && k[0].x < words;
@@ -414,17 +445,10 @@ __global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pa
       for (int q = 0; q < V; ++q) sum[q] = from[threadIdx.x * V + q];
       bool on = role || (one && out);  // the run reaches the next stretch
       if (on) {
-        // the run's last piece here: that of the first group behind this one which it does not pass through
-        int e = groups;
-        const int t0 = (g + 1) << lg;  // (thread 256 is none: the last group's run leaves the span)
-        for (int w = t0 >> 6; w < 4 && e == groups; ++w) {
-          const unsigned long long stop = ~through[w] & (w == t0 >> 6 ? ~0ull << (t0 & 63) : ~0ull);
-          if (stop) e = (w * 64 + __ffsll(stop) - 1) >> lg;
-        }
+        const int e = first_stop(g + 1);
         on = e == groups;
-        const int n1 = min(e + 1, groups);
-        // in order, several pieces' reads at once (one by one, each behind its own flag, took this launch 17 us
-        // where it takes 12: 8955 x 24 fp16 over 56 words; more at once take registers that waves need)
+        // in order, several pieces' reads at once (more at once take registers that waves need)
+        const int n1 = min((TREE ? g + 1 : e) + 1, groups);
         for (int j = g + 1; j < n1; j += kAt) {
           float x[kAt][V];
 #pragma unroll
@@ -457,20 +481,22 @@ __global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pa
 // of few spans is summed at once; a longer one is left to the whole workgroup, whose groups take equal
 // stretches of it and join them through LDS, so that half a list of one token is no chain of loads.
 constexpr int kShort = 8;
+constexpr int kOwned = 8;  // spans a workgroup looks after: its long runs follow each other
 
 template <int V>
 __global__ __launch_bounds__(256) void k_grad_join(const uint2* __restrict__ pairs, int64_t n, int64_t spans, int S,
                                                    unsigned words, int E, float scale, const float* __restrict__ part,
                                                    float* __restrict__ dtable, int lg) {
   const int G = 1 << lg, groups = 256 >> lg, grp = threadIdx.x >> lg, lane = threadIdx.x & (G - 1);
+  const int owned = min(groups, kOwned);  // spans of this workgroup
   __shared__ float red[256 * V];
   __shared__ int64_t longs[256];
   __shared__ int nlong;
   if (threadIdx.x == 0) nlong = 0;
   __syncthreads();
-  const int64_t s = (int64_t)blockIdx.x * groups + grp;
+  const int64_t s = (int64_t)blockIdx.x * owned + grp;
   const int64_t end = (s + 1) * S;  // the next span's first entry
-  if (end < n) {
+  if (grp < owned && end < n) {
     // all the keys that decide, asked for together: the span's ends, the entry in front of it, and the
     // first entries of the next spans
     const unsigned cur = pairs[end].x, tail = pairs[end - 1].x, head = pairs[s * S].x;
@@ -546,14 +572,17 @@ __global__ __launch_bounds__(256) void k_grad_join(const uint2* __restrict__ pai
       }
 #pragma unroll
       for (int q = 0; q < V; ++q) red[q * 256 + threadIdx.x] = acc[q];
-      __syncthreads();
+      const int used = (int)((cnt + per - 1) / per);
+      for (int d = 1; d < used; d <<= 1) {
+        __syncthreads();
+        if (!(grp & (2 * d - 1)) && grp + d < used)
+#pragma unroll
+          for (int q = 0; q < V; ++q) red[q * 256 + threadIdx.x] += red[q * 256 + threadIdx.x + (d << lg)];
+      }
       if (grp == 0 && c < E) {
         Pack<float, V> x = ldv<float, V>(part + (2 * h + 1) * E + c);
-        for (int g = 0; g < groups; ++g)
 #pragma unroll
-          for (int q = 0; q < V; ++q) x.v[q] += red[q * 256 + (g << lg) + lane];
-#pragma unroll
-        for (int q = 0; q < V; ++q) x.v[q] *= scale;
+        for (int q = 0; q < V; ++q) x.v[q] = (x.v[q] + red[q * 256 + threadIdx.x]) * scale;
         stv<float, V>(dtable + (int64_t)tok * E + c, x);
       }
       __syncthreads();
@@ -665,7 +694,7 @@ GradWs grad_ws(int64_t n, int64_t V, int E, int dtype) {
   int bits = 1;
   while (((int64_t)1 << bits) <= V) ++bits;  // keys 0 .. V
   g.passes = (bits + 9) / 10;
-  g.bits = std::max(2, (bits + g.passes - 1) / g.passes);
+  g.bits = std::max(6, (bits + g.passes - 1) / g.passes);  // (few bins leave k_sort_place long sums for few threads)
   const int64_t t1 = (n + 1023) / 1024;
   g.items = (t1 << g.bits) <= kOwnSums ? 1 : 4;
   g.tiles = (n + 1024 * g.items - 1) / (1024 * g.items);
@@ -760,14 +789,22 @@ int run_grad(const void* dy, int dtype, int64_t lddy, const I* ids, int64_t n, i
       else pass(std::integral_constant<int, 4>{});
     }
   }
-  auto blocks_of = [&](int lg) { return dim3((unsigned)((g.spans + (256 >> lg) - 1) / (256 >> lg))); };
+  auto blocks_of = [&](int lg) { 
+    const int owned = std::min(256 >> lg, kOwned);
+    return dim3((unsigned)((g.spans + owned - 1) / owned));
+  };
   by_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
     by_cols_of(cols_of(E, kGradCols<T>), [&](auto vec) {
       constexpr int VEC = decltype(vec)::value;
-      if constexpr (VEC <= kGradCols<T>)
-        hipLaunchKernelGGL((k_grad_spans<T, VEC>), dim3((unsigned)g.spans), dim3(256), 0, s, pairs[side], n, (unsigned)V,
-                           (const T*)dy, lddy, E, scale, dtable, part, lanes_log2(E, VEC));
+      if constexpr (VEC <= kGradCols<T>) {
+        const int lg = lanes_log2(E, VEC);
+        // 32 stretches a span and more add their pieces up by doubling (175517 x 4 bf16 over 25 words 22 us for this
+        // launch, 9.6 by doubling), fewer one after the other (196608 x 128 over 21128: 18.7 us, 20.5 by doubling)
+        auto kernel = lg <= 3 ? k_grad_spans<T, VEC, true> : k_grad_spans<T, VEC, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)g.spans), dim3(256), 0, s, pairs[side], n, (unsigned)V, (const T*)dy, lddy, E,
+                           scale, dtable, part, lg);
+      }
     });
   });
   if (g.spans > 1) {
