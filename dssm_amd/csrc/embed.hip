@@ -15,8 +15,8 @@
 // are written by extra workgroups of the sort's launches, whose own work is latency.
 //
 // Measured, 196608 tokens of 128 columns over 21128 words (log-uniform; 62 MB that must move, 12.7 us at the
-// rate of a large copy): lookup fp32 -> bf16 14.3 us, 4.3 TB/s; gradient of bf16 rows 49 us in six launches:
-// per digit count 3.2 and place 8.8 us (loads, tile sums and ranks one behind the other: latency), spans 19
+// rate of a large copy): lookup fp32 -> bf16 14.3 us, 4.3 TB/s; gradient of bf16 rows 47 us in six launches:
+// per digit count 3.2 and place 8.8 us (loads, tile sums and ranks one behind the other: latency), spans 18
 // (50 MB of gathered rows, every workgroup resident at once: the rows' own time and two latencies), join 6.
 #include <hip/hip_runtime.h>
 
