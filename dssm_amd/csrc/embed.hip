@@ -799,9 +799,10 @@ int run_grad(const void* dy, int dtype, int64_t lddy, const I* ids, int64_t n, i
       constexpr int VEC = decltype(vec)::value;
       if constexpr (VEC <= kGradCols<T>) {
         const int lg = lanes_log2(E, VEC);
-        // 32 stretches a span and more add their pieces up by doubling (175517 x 4 bf16 over 25 words 22 us for this
-        // launch, 9.6 by doubling), fewer one after the other (196608 x 128 over 21128: 18.7 us, 20.5 by doubling)
-        auto kernel = lg <= 3 ? k_grad_spans<T, VEC, true> : k_grad_spans<T, VEC, false>;
+        // 64 stretches a span and more add their pieces up by doubling (175517 x 4 bf16 over 25 words 22 us for this
+        // launch, 9.6 by doubling; the whole gradient of 196608 x 32 bf16 over 500 words 32.5 and 29.3), fewer one after
+        // the other (196608 x 32 fp32 28.5 and 29.1, 196608 x 128 bf16 over 21128 words 18.4 us for this launch and 20.5)
+        auto kernel = lg <= 2 ? k_grad_spans<T, VEC, true> : k_grad_spans<T, VEC, false>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)g.spans), dim3(256), 0, s, pairs[side], n, (unsigned)V, (const T*)dy, lddy, E,
                            scale, dtable, part, lg);
       }
