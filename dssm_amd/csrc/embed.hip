@@ -30,10 +30,10 @@ namespace seq {
 namespace {
 
 // ---- lookup ------------------------------------------------------------------------------------
-// A lane owns V neighbouring columns (8, 4 or 1: the widest that divides E, so that every access is whole),
-// a row takes G lanes (a power of two up to 64, wider rows loop) and a wave 64 / G rows.  A row is one
-// dependent gather behind its id, so each lane has kLookRows rows in flight: the ids first, then the rows
-// as they are, converted only when all have been asked for.
+// A lane owns V neighbouring columns (cols_of; the last lane of a row whose width is no multiple takes the row's last
+// V, and both that own a column store the same), a row takes G lanes (a power of two up to 64, wider rows loop) and
+// a wave 64 / G rows.  A row is one dependent gather behind its id, so each lane has kLookRows rows in flight: the
+// ids first, then the rows as they are, converted only when all have been asked for.
 constexpr int kLookRows = 4;
 
 template <typename T, typename O, typename I, int V>
@@ -48,7 +48,8 @@ __global__ __launch_bounds__(256) void k_lookup(const T* __restrict__ table, int
     const int64_t r = r0 + (int64_t)j * slots;
     id[j] = r < n ? (int64_t)ids[r] : -1;
   }
-  for (int c = (threadIdx.x & (G - 1)) * V; c < E; c += G * V) {
+  for (int c0 = (threadIdx.x & (G - 1)) * V; c0 < E; c0 += G * V) {
+    const int c = min(c0, E - V);
     Pack<T, V> x[kLookRows];
 #pragma unroll
     for (int j = 0; j < kLookRows; ++j)
@@ -378,8 +379,8 @@ __global__ __launch_bounds__(256) void k_grad_spans(const uint2* __restrict__ pa
     return e;
   };
   for (int c0 = 0; c0 < E; c0 += G * V) {
-    const int c = c0 + lane * V;
-    const bool mine = c < E;
+    const bool mine = c0 + lane * V < E;
+    const int c = min(c0 + lane * V, E - V);
     Pack<T, V> x[kStretch];
 #pragma unroll
     for (int j = 0; j < kStretch; ++j)
@@ -510,7 +511,8 @@ __global__ __launch_bounds__(256) void k_grad_join(const uint2* __restrict__ pai
 #pragma unroll
       for (int j = 0; j < kShort; ++j) more += more == j && ahead[j] == cur;
       if (more < kShort) {
-        for (int c = lane * V; c < E; c += G * V) {
+        for (int c0 = lane * V; c0 < E; c0 += G * V) {
+          const int c = min(c0, E - V);
           Pack<float, V> x[kShort + 1];
           x[0] = ldv<float, V>(part + (2 * s + 1) * E + c);
 #pragma unroll
@@ -549,11 +551,12 @@ __global__ __launch_bounds__(256) void k_grad_join(const uint2* __restrict__ pai
     const int64_t cnt = lo - h, per = (cnt + groups - 1) / groups;
     const int64_t a = min(h + 1 + grp * per, lo + 1), b = min(a + per, lo + 1);
     for (int c0 = 0; c0 < E; c0 += G * V) {
-      const int c = c0 + lane * V;
+      const bool mine = c0 + lane * V < E;
+      const int c = min(c0 + lane * V, E - V);
       float acc[V];
 #pragma unroll
       for (int q = 0; q < V; ++q) acc[q] = 0.f;
-      if (c < E) {
+      if (mine) {
         int64_t t = a;
         for (; t + 8 <= b; t += 8) {
           Pack<float, V> x[8];
@@ -579,7 +582,7 @@ __global__ __launch_bounds__(256) void k_grad_join(const uint2* __restrict__ pai
 #pragma unroll
           for (int q = 0; q < V; ++q) red[q * 256 + threadIdx.x] += red[q * 256 + threadIdx.x + (d << lg)];
       }
-      if (grp == 0 && c < E) {
+      if (grp == 0 && mine) {
         Pack<float, V> x = ldv<float, V>(part + (2 * h + 1) * E + c);
 #pragma unroll
         for (int q = 0; q < V; ++q) x.v[q] = (x.v[q] + red[q * 256 + threadIdx.x]) * scale;
@@ -659,8 +662,15 @@ __global__ __launch_bounds__(256) void k_grad_few(const I* __restrict__ ids, int
   for (int i = threadIdx.x; i < total; i += 256) out[i] = acc[i] * scale;
 }
 
-// Columns a lane owns: the widest of 8, 4 and 1 that divides a row, `most` at most.
-int cols_of(int E, int most) { return most >= 8 && E % 8 == 0 ? 8 : E % 4 == 0 ? 4 : 1; }
+// Columns a lane owns: 8, 4 or 1, `most` at most; the widest that divides the row or leaves it four lanes (196608 ids over
+// 21128 words: 118 bf16 columns 12.6 us and 49, their gradient, with 8 a lane, 26.6 and 69 with one; 33 fp32 9.9 and 44,
+// 16.5 and 53; but 20000 ids, 11 bf16 columns 3.4 and 25.6 with 8 a lane, 2.9 and 23.5 with one).  k_grad_few, which adds
+// up in place, takes the widest that divides the row.
+int cols_of(int E, int most) {
+  if (most >= 8 && (E % 8 == 0 || E >= 32)) return 8;
+  return E % 4 == 0 || E >= 16 ? 4 : 1;
+}
+int divisor_of(int E, int most) { return most >= 8 && E % 8 == 0 ? 8 : E % 4 == 0 ? 4 : 1; }
 template <typename F>
 void by_cols_of(int v, F&& f) {
   if (v == 8) f(std::integral_constant<int, 8>{});
@@ -731,7 +741,7 @@ int run_grad(const void* dy, int dtype, int64_t lddy, const I* ids, int64_t n, i
     const int RR = (int)std::max<int64_t>(1, std::min<int64_t>(kFewLds / 4 / E, (V + 2047) / 2048));
     by_dtype(dtype, [&](auto tag) {
       using T = decltype(tag);
-      by_cols_of(cols_of(E, kGradCols<T>), [&](auto vec) {
+      by_cols_of(divisor_of(E, kGradCols<T>), [&](auto vec) {
         constexpr int VEC = decltype(vec)::value;
         if constexpr (VEC <= kGradCols<T>)
           hipLaunchKernelGGL((k_grad_few<T, I, VEC>), dim3((unsigned)((V + RR - 1) / RR)), dim3(256), (size_t)RR * E * 4, s, ids,

@@ -32,7 +32,8 @@ def rounded(got, want, tol):
 
 # ---- embedding ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,out", [(F32, BF), (F32, F32), (BF, BF), (F16, F32), (BF, F16), (F32, F16)])
-@pytest.mark.parametrize("n,V,E", [(1, 1, 1), (3, 7, 4), (77, 50, 33), (130, 1000, 128), (5, 9, 513), (1031, 300, 100)])
+@pytest.mark.parametrize("n,V,E", [(1, 1, 1), (3, 7, 4), (77, 50, 33), (130, 1000, 128), (5, 9, 513), (1031, 300, 100),
+                                   (300, 20, 17), (90, 40, 131), (60, 8, 39), (50, 9, 11)])
 def test_lookup(device, n, V, E, dtype, out):
     g = gen(n * 1000 + E)
     table = torch.randn(V, E, generator=g).to(dtype)
@@ -74,6 +75,7 @@ def check_grad(device, dy, ids, V, scale=0.5):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,V,E", [(1, 1, 1), (2, 5, 3), (31, 3, 8), (32, 3, 8), (33, 1, 7), (64, 2, 16), (100, 1, 1), (1000, 40, 100),
                                    (4096, 700, 20), (4097, 700, 20), (5000, 1023, 9), (9000, 1024, 5), (12345, 70000, 12),
+                                   (5000, 300, 33), (3000, 200, 131), (2000, 90, 17), (700, 60, 513), (6000, 7, 39),
                                    (3, 1 << 21, 2)])
 def test_lookup_grad(device, n, V, E, dtype):
     g = gen(n + V + E)
