@@ -545,7 +545,7 @@ Cut cut_of(int64_t R, int T, int H, int dtype) {
 }
 
 bool recur_dims_ok(int64_t R, int T, int H) {
-  return R > 0 && T > 0 && H > 0 && T <= (1 << 28) && H <= (1 << 20) && R <= ((int64_t)1 << 31) &&
+  return R >= 0 && T > 0 && H > 0 && T <= (1 << 28) && H <= (1 << 20) && R <= ((int64_t)1 << 31) &&
          R * H <= ((int64_t)1 << 31);  // (a lane a state: a launch has fewer than 2^32 threads)
 }
 
@@ -602,7 +602,7 @@ int run(RecurArgs& a, int dtype, void* stream) {
 using namespace dssm::seq;
 
 extern "C" size_t dssm_linear_recurrence_ws_bytes(int64_t R, int T, int H, int dtype) {
-  if (!recur_dims_ok(R, T, H) || !seq_dtype(dtype)) return 0;
+  if (!recur_dims_ok(R, T, H) || !seq_dtype(dtype) || R == 0) return 0;
   const Cut c = cut_of(R, T, H, dtype);
   return c.S > 1 ? (size_t)2 * c.S * R * H * sizeof(float) : 0;
 }
@@ -611,8 +611,9 @@ extern "C" int dssm_linear_recurrence(const void* gate, int64_t gr, int64_t gt, 
                                       int dtype, const int32_t* lens, const float* h0, int64_t R, int T, int H,
                                       int reverse, void* h, int64_t hr, int64_t ht, float* last, float* states, void* ws,
                                       size_t ws_bytes, void* stream) {
-  if (!gate || !cand || !h || !last || !seq_dtype(dtype) || !recur_dims_ok(R, T, H))
+  if (!seq_dtype(dtype) || !recur_dims_ok(R, T, H) || (R > 0 && (!gate || !cand || !h || !last)))
     return dssm::report_error(DSSM_E_INVALID, "linear_recurrence: bad argument");
+  if (R == 0) return DSSM_OK;
   const size_t need = dssm_linear_recurrence_ws_bytes(R, T, H, dtype);
   if (need && (!ws || ws_bytes < need))
     return dssm::report_error(DSSM_E_INVALID, "linear_recurrence: workspace too small (dssm_linear_recurrence_ws_bytes)");
@@ -643,8 +644,9 @@ extern "C" int dssm_linear_recurrence_bwd(const void* gate, int64_t gr, int64_t 
                                           int64_t dr, int64_t dt, const float* dlast, int64_t R, int T, int H, int reverse,
                                           void* dgate, int64_t ogr, int64_t ogt, void* dcand, int64_t ocr, int64_t oct,
                                           float* dh0, void* ws, size_t ws_bytes, void* stream) {
-  if (!gate || !cand || !states || !dgate || !dcand || !seq_dtype(dtype) || !recur_dims_ok(R, T, H))
+  if (!seq_dtype(dtype) || !recur_dims_ok(R, T, H) || (R > 0 && (!gate || !cand || !states || !dgate || !dcand)))
     return dssm::report_error(DSSM_E_INVALID, "linear_recurrence_bwd: bad argument");
+  if (R == 0) return DSSM_OK;
   const size_t need = dssm_linear_recurrence_ws_bytes(R, T, H, dtype);
   if (need && (!ws || ws_bytes < need))
     return dssm::report_error(DSSM_E_INVALID, "linear_recurrence_bwd: workspace too small (dssm_linear_recurrence_ws_bytes)");
@@ -678,8 +680,9 @@ extern "C" int dssm_linear_recurrence_bwd(const void* gate, int64_t gr, int64_t 
 
 extern "C" int dssm_linear_recurrence_step(const void* gate, int64_t gr, const void* cand, int64_t cr, int dtype,
                                            float* state, int64_t sr, void* h, int64_t hr, int64_t R, int H, void* stream) {
-  if (!gate || !cand || !state || !h || !seq_dtype(dtype) || !recur_dims_ok(R, 1, H))
+  if (!seq_dtype(dtype) || !recur_dims_ok(R, 1, H) || (R > 0 && (!gate || !cand || !state || !h)))
     return dssm::report_error(DSSM_E_INVALID, "linear_recurrence_step: bad argument");
+  if (R == 0) return DSSM_OK;
   by_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
     auto go = [&](auto vec) {

@@ -695,7 +695,8 @@ int dssm_rnn_adam_ex(float* p, const float* g, float* m, float* v, int64_t n_spa
  * lookup, a recurrence whose gates do not look at the state (so that time can be cut), the norm between
  * layers, and the 8-bit product.  Storage types dtype / out_dtype: DSSM_F32, DSSM_BF16, DSSM_F16; sums,
  * statistics and states are fp32.  Leading dimensions and strides are in elements, rows may start at any
- * element.  Sizes of zero rows do nothing.  Outputs must not overlap inputs unless a call says so. */
+ * element.  Sizes of zero rows do nothing, and pointers to such rows may be NULL (gradients that are sums over rows are
+ * zeros).  Outputs must not overlap inputs unless a call says so. */
 
 /* tf.nn.embedding_lookup(table, ids) * scale (dssm_rnn.py:113-118): out [n x E] from table [V x E] (row
  * stride ldt).  ids: int32, or int64 with ids64; an id outside [0, V) gives a row of zeros. */
@@ -716,7 +717,7 @@ int dssm_embedding_grad(const void* dy, int dtype, int64_t lddy, const void* ids
  * first.  h0 [R x H] fp32 or NULL (zeros); last [R x H] fp32: the state after the walk.  states (NULL for
  * inference): ceil(T / DSSM_RECUR_PIECE) x R x H floats, the state in front of every DSSM_RECUR_PIECE steps of
  * the walk, read by the backward.  ws: dssm_linear_recurrence_ws_bytes() bytes of any content (0: none
- * is needed, ws may be NULL); forward and backward need the same.  T <= 2^28, H <= 2^20, R * H <= 2^31. */
+ * is needed, ws may be NULL); forward and backward need the same.  1 <= T <= 2^28, 1 <= H <= 2^20, R * H <= 2^31. */
 #define DSSM_RECUR_PIECE 8
 size_t dssm_linear_recurrence_ws_bytes(int64_t R, int T, int H, int dtype);
 int dssm_linear_recurrence(const void* gate, int64_t gate_row, int64_t gate_time, const void* cand, int64_t cand_row,
