@@ -363,6 +363,7 @@ void by_cols(int cols, F&& f) {
 bool norm_dims_ok(int64_t rows, int cols) {
   return rows >= 0 && rows <= 0x7fffffff && cols > 0 && cols <= kMaxCols;
 }
+bool eps_ok(float eps) { return eps > 0.f && eps < __builtin_inff(); }
 int kp_of(int cols) { return (cols + kBlk - 1) / kBlk * kBlk; }
 
 template <int MODE>
@@ -396,9 +397,9 @@ using namespace dssm::seq;
 extern "C" int dssm_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldres, const float* weight,
                              int64_t rows, int cols, int dtype, float eps, void* y, int64_t ldy, void* s, int64_t lds,
                              float* rstd, void* stream) {
-  if (!seq_dtype(dtype) || !norm_dims_ok(rows, cols) || !weight || ldx < cols || ldy < cols || (residual && ldres < cols) ||
-      (s && lds < cols) || (rows > 0 && (!x || !y)))
-    return dssm::report_error(DSSM_E_INVALID, "rms_norm: bad argument (1 to 16384 columns)");
+  if (!seq_dtype(dtype) || !norm_dims_ok(rows, cols) || !eps_ok(eps) || !weight || ldx < cols || ldy < cols ||
+      (residual && ldres < cols) || (s && lds < cols) || (rows > 0 && (!x || !y)))
+    return dssm::report_error(DSSM_E_INVALID, "rms_norm: bad argument (1 to 16384 columns, a positive finite eps)");
   if (rows == 0) return DSSM_OK;
   NormArgs a{};
   a.x = x;
@@ -421,9 +422,10 @@ extern "C" int dssm_rms_norm(const void* x, int64_t ldx, const void* residual, i
 extern "C" int dssm_rms_norm_blocks8(const void* x, int64_t ldx, const void* residual, int64_t ldres, const float* weight,
                                      int64_t rows, int cols, int dtype, float eps, void* q, void* scale, void* s,
                                      int64_t lds, float* rstd, void* stream) {
-  if (!seq_dtype(dtype) || !norm_dims_ok(rows, cols) || !weight || ldx < cols || (residual && ldres < cols) ||
+  if (!seq_dtype(dtype) || !norm_dims_ok(rows, cols) || !eps_ok(eps) || !weight || ldx < cols || (residual && ldres < cols) ||
       (s && lds < cols) || (rows > 0 && (!x || !q || !scale)) || (uintptr_t)q % 16)
-    return dssm::report_error(DSSM_E_INVALID, "rms_norm_blocks8: bad argument (1 to 16384 columns, 16-byte aligned values)");
+    return dssm::report_error(DSSM_E_INVALID,
+                              "rms_norm_blocks8: bad argument (1 to 16384 columns, a positive finite eps, 16-byte aligned values)");
   if (rows == 0) return DSSM_OK;
   NormArgs a{};
   a.x = x;

@@ -18,7 +18,6 @@ can be captured into a graph.  Wrong types and shapes raise TypeError / ValueErr
 """
 from __future__ import annotations
 
-import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -28,6 +27,8 @@ from . import _lib
 _CODE = {torch.float32: _lib.DSSM_F32, torch.bfloat16: _lib.DSSM_BF16, torch.float16: _lib.DSSM_F16}
 BLOCK = 128          # columns that share a scale
 MAX_NORM_COLS = 16384
+# what rounds to a positive finite float32 lies between these
+_EPS_LOW, _EPS_HIGH = 2.0 ** -150, 2.0 ** 128 - 2.0 ** 103
 _PIECE = 8           # include/dssm.h DSSM_RECUR_PIECE
 
 
@@ -278,8 +279,8 @@ def _norm_args(x, weight, residual, eps):
         raise ValueError(f"x must have 1 to {MAX_NORM_COLS} columns")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("residual must have x's shape and type")
-    if not (eps > 0 and math.isfinite(eps)):
-        raise ValueError("eps must be positive")
+    if not _EPS_LOW < eps < _EPS_HIGH:
+        raise ValueError("eps must be positive and finite as a float32")
     return code, _vector(weight, x.shape[-1], "weight")
 
 

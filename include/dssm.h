@@ -738,7 +738,8 @@ int dssm_linear_recurrence_step(const void* gate, int64_t ldgate, const void* ca
 
 /* Root-mean-square norm of s = x + residual (rounded to dtype; residual NULL: s = x): rstd = 1 /
  * sqrt(mean s^2 + eps), y = s * rstd * weight.  s (NULL: not wanted; may be x or residual itself) and rstd
- * [rows] (NULL: not wanted) are what the backward reads.  weight [cols] fp32, 1 to 16384 columns. */
+ * [rows] (NULL: not wanted) are what the backward reads.  weight [cols] fp32, 1 to 16384 columns, eps positive and
+ * finite. */
 int dssm_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldres, const float* weight, int64_t rows,
                   int cols, int dtype, float eps, void* y, int64_t ldy, void* s, int64_t lds, float* rstd, void* stream);
 /* Gradient: dx (= d residual) = the norm's gradient of dy at s, plus ds (NULL: none; the gradient that

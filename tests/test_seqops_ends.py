@@ -22,3 +22,21 @@ def test_zero_rows_do_nothing():
     assert lib.dssm_linear_recurrence(0, 0, 4, 0, 0, 4, F32, 0, 0, 0, 3, 0, 0, 0, 0, 4, 0, 0, 0, 0, 0) == -1
     assert lib.dssm_linear_recurrence_step(0, 4, 0, 4, 7, 0, 4, 0, 4, 0, 4, 0) == -1
     assert lib.dssm_linear_recurrence_step(P, 4, P, 4, F32, P, 4, P, 4, -1, 4, 0) == -1
+
+
+@pytest.mark.parametrize("eps", [0.0, -1e-6, float("nan"), float("inf"), 2.0 ** -150, 1e-46, 3.5e38])
+def test_eps_is_positive_as_a_float32(eps):
+    """An eps that is 0 as fp32 would make a row of zeros NaN."""
+    for call in (api.rms_norm, api.rms_norm_blocks8):
+        with pytest.raises(ValueError, match="eps"):
+            call(Z(3, 4), Z(4), None, eps)
+    lib = _lib.load()
+    assert lib.dssm_rms_norm(0, 4, 0, 0, P, 0, 4, F32, eps, 0, 4, 0, 0, 0, 0) == -1
+    assert lib.dssm_rms_norm_blocks8(0, 4, 0, 0, P, 0, 4, F32, eps, 0, 0, 0, 0, 0, 0) == -1
+
+
+@pytest.mark.parametrize("eps", [1e-45, 1e-6, 3.4e38])
+def test_eps_that_a_float32_holds_is_taken(eps):
+    with pytest.raises(ValueError, match="GPU"):  # past the check of eps, to the one of the device
+        api.rms_norm(Z(3, 4), Z(4), None, eps)
+    assert _lib.load().dssm_rms_norm(0, 4, 0, 0, P, 0, 4, F32, eps, 0, 4, 0, 0, 0, 0) == 0
