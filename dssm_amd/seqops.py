@@ -27,6 +27,7 @@ from . import _lib
 _CODE = {torch.float32: _lib.DSSM_F32, torch.bfloat16: _lib.DSSM_BF16, torch.float16: _lib.DSSM_F16}
 BLOCK = 128          # columns that share a scale
 MAX_NORM_COLS = 16384
+MAX_BLOCKS8_COLS = 1 << 22
 # what rounds to a positive finite float32 lies between these
 _EPS_LOW, _EPS_HIGH = 2.0 ** -150, 2.0 ** 128 - 2.0 ** 103
 _PIECE = 8           # include/dssm.h DSSM_RECUR_PIECE
@@ -375,8 +376,8 @@ def quantize_blocks8(x: torch.Tensor) -> Blocks8:
     two that brings their largest finite magnitude into e4m3's +-448 (1 for a block of zeros); values round
     to nearest even, NaN and infinities become NaN.  Weights [N x K] are laid out once with this."""
     code = _code(x.dtype, "x")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_NORM_COLS:
-        raise ValueError(f"x must have 1 to {MAX_NORM_COLS} columns")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_BLOCKS8_COLS:
+        raise ValueError(f"x must have 1 to {MAX_BLOCKS8_COLS} columns")
     dev = _on_gpu(x)
     x2, ld = _rows(x)
     b = _empty8(x2.shape[0], x.shape[-1], dev)
@@ -391,8 +392,8 @@ def dequantize_blocks8(b: Blocks8, dtype: torch.dtype = torch.float32) -> torch.
     normal magnitude)."""
     code = _code(dtype, "dtype")
     rows = _check8(b, "b")
-    if b.cols > MAX_NORM_COLS:
-        raise ValueError(f"b must have 1 to {MAX_NORM_COLS} columns")
+    if b.cols > MAX_BLOCKS8_COLS:
+        raise ValueError(f"b must have 1 to {MAX_BLOCKS8_COLS} columns")
     dev = _on_gpu(b.q, b.scale)
     out = _empty(rows, b.cols, dtype=dtype, device=dev)
     if rows:
@@ -412,7 +413,7 @@ def blocks8_matmul(a: Blocks8, w: Blocks8, bias: Optional[torch.Tensor] = None,
     M, N = _check8(a, "a"), _check8(w, "w")
     if a.cols != w.cols:
         raise ValueError(f"a has {a.cols} columns, w {w.cols}")
-    if M > 1 << 28 or N > 1 << 24 or a.cols > 1 << 22:
+    if M > 1 << 28 or N > 1 << 24 or a.cols > MAX_BLOCKS8_COLS:
         raise ValueError("at most 2^28 rows, 2^24 outputs and 2^22 columns")
     bias = _vector(bias, N, "bias")
     dev = _on_gpu(a.q, a.scale, w.q, w.scale, bias)

@@ -752,7 +752,7 @@ int dssm_rms_norm_bwd(const void* dy, int64_t lddy, const void* s, int64_t lds, 
 /* The 8-bit block form of [rows x K]: q [rows x Kp] e4m3 (Kp = K rounded up to 128, padding zero, 16-byte
  * aligned) and scale [rows x Kp / 128] E8M0 bytes: a row's block of 128 columns stands for q * 2^(byte -
  * 127), the smallest power of two that brings the block's largest finite magnitude into +-448 (2^0 for a
- * block of zeros).  Values round to nearest even; NaN and infinities become NaN. */
+ * block of zeros).  Values round to nearest even; NaN and infinities become NaN.  1 to 2^22 columns. */
 int dssm_quantize_blocks8(const void* x, int64_t ldx, int64_t rows, int cols, int dtype, void* q, void* scale, void* stream);
 int dssm_dequantize_blocks8(const void* q, const void* scale, int64_t rows, int cols, void* out, int64_t ldo, int out_dtype,
                             void* stream);

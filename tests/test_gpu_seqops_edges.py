@@ -5,7 +5,7 @@ import torch
 
 from dssm_amd import api
 from tests import seqops_ref as ref
-from tests.test_gpu_seqops import BF, F16, F32, gen, inputs, near, rounded
+from tests.test_gpu_seqops import BF, F16, F32, check_blocks, gen, inputs, near, product, rounded
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -48,3 +48,34 @@ def test_infinite_states_stay_infinite(device, R, T, H, dtype, reverse):
     same_ends(dg, wg, eg)
     same_ends(dc, wc, ec)
     same_ends(d0, w0, e0)
+
+
+# ---- 8-bit form --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("rows,cols", [(3, 16385), (2, 16384 * 2), (700, 16391), (2, 40000), (1, 16384 * 3 + 129)])
+def test_rows_wider_than_the_norms(device, rows, cols, dtype):
+    """The 8-bit form of rows of more than 16384 columns, between rows' ends that are NaN."""
+    g = gen(rows * cols)
+    x = (torch.randn(rows, cols, generator=g) * torch.exp(2 * torch.randn(rows, 1, generator=g))).to(dtype)
+    x[0, 16384:16512] = 0  # the first block behind a stretch
+    x[rows - 1, :128] = 2.0 ** -12
+    around = torch.full((rows, cols + 9), float("nan"), dtype=dtype, device=device)
+    around[:, 5:5 + cols] = x.to(device)
+    b = api.quantize_blocks8(around[:, 5:5 + cols])
+    check_blocks(b, x.double(), torch.zeros(rows, cols, dtype=torch.float64))
+    # block by block it is what rows of the norm's width have
+    for c0 in range(0, cols, 16384):
+        part = api.quantize_blocks8(x[:, c0:c0 + 16384].contiguous().to(device))
+        kp = part.q.shape[1]
+        assert torch.equal(part.q.view(torch.uint8), b.q.view(torch.uint8)[:, c0:c0 + kp])
+        assert torch.equal(part.scale.view(torch.uint8), b.scale.view(torch.uint8)[:, c0 // 128:(c0 + kp) // 128])
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 40, 20000), (130, 300, 16384 + 77), (600, 700, 33000)])
+def test_product_of_wide_rows(device, M, N, K):
+    g = gen(K)
+    a = api.quantize_blocks8(torch.randn(M, K, generator=g).to(device))
+    w = api.quantize_blocks8((torch.randn(N, K, generator=g) * K ** -0.5).to(device))
+    bias = torch.randn(N, generator=g)
+    want, tol = product(a, w, bias, K)
+    rounded(api.blocks8_matmul(a, w, bias.to(device)), want, tol)

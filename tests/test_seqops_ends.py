@@ -40,3 +40,20 @@ def test_eps_that_a_float32_holds_is_taken(eps):
     with pytest.raises(ValueError, match="GPU"):  # past the check of eps, to the one of the device
         api.rms_norm(Z(3, 4), Z(4), None, eps)
     assert _lib.load().dssm_rms_norm(0, 4, 0, 0, P, 0, 4, F32, eps, 0, 4, 0, 0, 0, 0) == 0
+
+
+def test_the_8_bit_form_is_as_wide_as_the_product():
+    """Rows that blocks8_matmul multiplies can be laid out: up to 2^22 columns, and no more."""
+    wide = Z(1, 1).expand(1, 1 << 22)
+    with pytest.raises(ValueError, match="GPU"):
+        api.quantize_blocks8(wide)
+    with pytest.raises(ValueError, match="columns"):
+        api.quantize_blocks8(Z(1, 1).expand(1, (1 << 22) + 1))
+    b = api.Blocks8(Z(1, 1 << 22, dtype=torch.uint8).view(torch.float8_e4m3fn),
+                    Z(1, 1 << 15, dtype=torch.uint8).view(torch.float8_e8m0fnu), 1 << 22)
+    with pytest.raises(ValueError, match="GPU"):
+        api.dequantize_blocks8(b)
+    lib = _lib.load()
+    for cols, rc in ((16385, 0), (1 << 22, 0), ((1 << 22) + 1, -1)):
+        assert lib.dssm_quantize_blocks8(0, cols, 0, cols, F32, 0, 0, 0) == rc
+        assert lib.dssm_dequantize_blocks8(0, 0, 0, cols, 0, cols, F32, 0) == rc
