@@ -838,9 +838,9 @@ using namespace dssm::seq;
 
 extern "C" int dssm_embedding_lookup(const void* table, int dtype, int64_t ldt, int64_t V, int E, const void* ids,
                                      int ids64, int64_t n, float scale, void* out, int out_dtype, void* stream) {
-  if (!table || !seq_dtype(dtype) || !seq_dtype(out_dtype) || V <= 0 || E <= 0 || ldt < E || n < 0 ||
+  if (!table || !seq_dtype(dtype) || !seq_dtype(out_dtype) || V <= 0 || E <= 0 || E > (1 << 30) || ldt < E || n < 0 ||
       (n > 0 && (!ids || !out)))
-    return dssm::report_error(DSSM_E_INVALID, "embedding_lookup: bad argument");
+    return dssm::report_error(DSSM_E_INVALID, "embedding_lookup: bad argument (1 to 2^30 columns)");
   if (n == 0) return DSSM_OK;
   const int v = cols_of(E, 8), lg = lanes_log2(E, v);
   const int64_t rows = (int64_t)(256 >> lg) * kLookRows, blocks = (n + rows - 1) / rows;

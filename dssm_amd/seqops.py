@@ -113,6 +113,8 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
     nothing and gives a row of zeros (a padding id, say)."""
     if table.dim() != 2 or 0 in table.shape:
         raise ValueError("table must be [V x E]")
+    if table.shape[1] > 1 << 30:
+        raise ValueError("at most 2^30 columns")
     out_dtype = table.dtype if dtype is None else dtype
     code, out_code = _code(table.dtype, "table"), _code(out_dtype, "dtype")
     ids = _ids(ids)
@@ -135,8 +137,8 @@ def embedding_grad(dy: torch.Tensor, ids: torch.Tensor, nwords: int, scale: floa
     if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] == 0:
         raise ValueError("dy must be [*ids.shape, E]")
     V, E, n = int(nwords), dy.shape[-1], ids.numel()
-    lib = _lib.load()
-    need = int(lib.dssm_embedding_grad_ws_bytes(n, V, E, code))
+    # (the query's answer for sizes that its arguments hold: they would be cut to 64 and 32 bits)
+    need = int(_lib.load().dssm_embedding_grad_ws_bytes(n, V, E, code)) if 0 < V < 1 << 30 and E <= 1 << 20 else 0
     if not need:
         raise ValueError(f"embedding_grad: {n} ids, {V} words, {E} columns are out of range "
                          "(fewer than 2^31 - 4096 ids, 1 to 2^30 - 1 words, 1 to 2^20 columns)")

@@ -699,7 +699,7 @@ int dssm_rnn_adam_ex(float* p, const float* g, float* m, float* v, int64_t n_spa
  * zeros).  Outputs must not overlap inputs unless a call says so. */
 
 /* tf.nn.embedding_lookup(table, ids) * scale (dssm_rnn.py:113-118): out [n x E] from table [V x E] (row
- * stride ldt).  ids: int32, or int64 with ids64; an id outside [0, V) gives a row of zeros. */
+ * stride ldt).  ids: int32, or int64 with ids64; an id outside [0, V) gives a row of zeros.  E <= 2^30. */
 int dssm_embedding_lookup(const void* table, int dtype, int64_t ldt, int64_t V, int E, const void* ids, int ids64,
                           int64_t n, float scale, void* out, int out_dtype, void* stream);
 /* Its gradient: dtable [V x E] fp32 (16-byte aligned, every row written) = scale * the rows of dy [n x E]

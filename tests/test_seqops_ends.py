@@ -57,3 +57,21 @@ def test_the_8_bit_form_is_as_wide_as_the_product():
     for cols, rc in ((16385, 0), (1 << 22, 0), ((1 << 22) + 1, -1)):
         assert lib.dssm_quantize_blocks8(0, cols, 0, cols, F32, 0, 0, 0) == rc
         assert lib.dssm_dequantize_blocks8(0, 0, 0, cols, 0, cols, F32, 0) == rc
+
+
+def test_sizes_that_an_int_would_cut_are_refused():
+    """2^32 + 4 columns are not 4."""
+    i = Z(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="columns"):
+        api.embedding_lookup(Z(1, 1).expand(5, (1 << 32) + 4), i)
+    with pytest.raises(ValueError, match="out of range"):
+        api.embedding_grad(Z(1, 1).expand(3, (1 << 32) + 4), i, 5)
+    with pytest.raises(ValueError, match="out of range"):
+        api.embedding_grad(Z(3, 4), i, (1 << 64) + 5)
+    with pytest.raises(ValueError, match="out of range"):
+        api.embedding_grad(Z(1, 1).expand(3, (1 << 20) + 1), i, 5)
+    with pytest.raises(ValueError, match="GPU"):
+        api.embedding_lookup(Z(1, 1).expand(5, 1 << 30), i)
+    # columns whose numbers would pass 2^31 on their way
+    assert _lib.load().dssm_embedding_lookup(P, F32, 2 ** 31 - 1, 4, 2 ** 31 - 1, 0, 0, 0, 1.0, 0, F32, 0) == -1
+    assert _lib.load().dssm_embedding_lookup(P, F32, 1 << 30, 4, 1 << 30, 0, 0, 0, 1.0, 0, F32, 0) == 0
