@@ -34,6 +34,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <cstdlib>
 #include <type_traits>
 
 #include "seq.h"
@@ -682,6 +683,8 @@ extern "C" int dssm_linear_recurrence_step(const void* gate, int64_t gr, const v
                                            float* state, int64_t sr, void* h, int64_t hr, int64_t R, int H, void* stream) {
   if (!seq_dtype(dtype) || !recur_dims_ok(R, 1, H) || (R > 0 && (!gate || !cand || !state || !h)))
     return dssm::report_error(DSSM_E_INVALID, "linear_recurrence_step: bad argument");
+  if (R > 1 && (std::abs(sr) < H || std::abs(hr) < H))
+    return dssm::report_error(DSSM_E_INVALID, "linear_recurrence_step: rows of state or h overlap");
   if (R == 0) return DSSM_OK;
   by_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);

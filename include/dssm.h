@@ -732,7 +732,8 @@ int dssm_linear_recurrence_bwd(const void* gate, int64_t gate_row, int64_t gate_
                                int64_t dh_row, int64_t dh_time, const float* dlast, int64_t R, int T, int H, int reverse,
                                void* dgate, int64_t dgate_row, int64_t dgate_time, void* dcand, int64_t dcand_row,
                                int64_t dcand_time, float* dh0, void* ws, size_t ws_bytes, void* stream);
-/* One step for R rows: state [R x H] fp32 in place, h [R x H] = the new state in the inputs' type. */
+/* One step for R rows: state [R x H] fp32 in place, h [R x H] = the new state in the inputs' type.  Rows of state, and
+ * of h, must not overlap each other. */
 int dssm_linear_recurrence_step(const void* gate, int64_t ldgate, const void* cand, int64_t ldcand, int dtype,
                                 float* state, int64_t ldstate, void* h, int64_t ldh, int64_t R, int H, void* stream);
 

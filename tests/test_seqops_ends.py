@@ -75,3 +75,12 @@ def test_sizes_that_an_int_would_cut_are_refused():
     # columns whose numbers would pass 2^31 on their way
     assert _lib.load().dssm_embedding_lookup(P, F32, 2 ** 31 - 1, 4, 2 ** 31 - 1, 0, 0, 0, 1.0, 0, F32, 0) == -1
     assert _lib.load().dssm_embedding_lookup(P, F32, 1 << 30, 4, 1 << 30, 0, 0, 0, 1.0, 0, F32, 0) == 0
+
+
+def test_a_steps_rows_that_overlap_are_refused():
+    """Two rows of one state would be moved on by two lanes at once."""
+    step = _lib.load().dssm_linear_recurrence_step
+    assert step(P, 4, P, 4, F32, P, 3, P, 4, 2, 4, 0) == -1
+    assert step(P, 4, P, 4, F32, P, 0, P, 4, 2, 4, 0) == -1
+    assert step(P, 4, P, 4, F32, P, 4, P, -3, 2, 4, 0) == -1
+    assert b"overlap" in _lib.load().dssm_last_error()
