@@ -5,7 +5,7 @@
 //   n = s rstd:  dx = rstd (w dy - n mean(w dy n)) + ds,   dw = sum over rows of dy n
 //
 // s is rounded to its storage type before the norm, so that the backward, which reads the stored s, is
-// the gradient of exactly this forward.  All sums are fp32.
+// the gradient of exactly this forward.  Sums are fp32, a row's squares 64 bits.
 //
 // Every kernel here is one pass over its rows, bound by memory.  A row stays in registers: NT threads (a
 // quarter wave to a workgroup of 16 waves) hold 8 neighbouring columns each, K times over; 16 lanes hold a
@@ -86,6 +86,35 @@ struct NormArgs {
   float eps;
 };
 
+// v becomes y = v up w (rstd + rest) in its first n columns, zeros behind them; up is a power of two.  E4M3: y is going
+// to be rounded to e4m3.
+template <bool E4M3>
+__device__ __forceinline__ void scale8(float (&v)[8], const float (&w)[8], float up, float rstd, float rest, int n) {
+  float y[8];
+  unsigned tie = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // with the product's rounding error and rstd's rest put back: rounded once
+    const float x = v[i] * up, p = x * w[i], e = fmaf(x, w[i], -p);
+    y[i] = i < n ? fmaf(p, rstd, fmaf(p, rest, e * rstd)) : 0.f;
+    tie |= (__float_as_uint(y[i]) & 0x7ffffu) == 0u;
+  }
+  if (E4M3 && tie) {
+    // y that lies half way between two e4m3 values (these have their last 19 bits clear; so have zeros) may have got
+    // there by its own rounding: it moves to the side that the exact value is on
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = v[i] * up, p = x * w[i], e = fmaf(x, w[i], -p);
+      const float d = fmaf(p, rstd, -y[i]) + fmaf(p, rest, e * rstd);
+      const unsigned u = __float_as_uint(y[i]);
+      if (i < n && (u & 0x7ffffu) == 0u && (u << 1) != 0u && (u << 1) < 0xff000000u && d != 0.f)
+        y[i] = __uint_as_float((d > 0.f) == (y[i] > 0.f) ? u + 1u : u - 1u);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = y[i];
+}
+
 // MODE 0: y in T; 1: y in the 8-bit form; 2: x itself in the 8-bit form (no norm).
 // A workgroup walks rows blockIdx.x * kRows + i * gridDim.x * kRows with the weights in registers and the next
 // rows' loads in flight behind the current ones' arithmetic.
@@ -94,11 +123,13 @@ struct NormArgs {
 template <typename T, int NT, int K, int MODE, bool R>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
   constexpr int kRows = NT < 256 ? 256 / NT : 1;
+  constexpr bool kBranch = MODE == 1 && sizeof(T) == 2;
   __shared__ double red[16];
   const int l = threadIdx.x % NT;
   const int64_t step = (int64_t)gridDim.x * kRows;
   const bool whole = a.cols >= 8;
   const int64_t ldq = a.kp;
+  bool heavy = false;  // one of this thread's weights is 2^64 or more
   if constexpr (MODE == 2 && NT * K * 8 == kMaxCols) {
     const int c0 = blockIdx.y * kMaxCols;
     a.x = (const T*)a.x + c0;
@@ -111,7 +142,11 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (k * NT + l) * 8, nv = a.cols - c;
-    if (MODE != 2 && nv > 0) ld_row<float, 8>(a.w + c, nv, w[k]);
+    if (MODE != 2 && nv > 0) {
+      ld_row<float, 8>(a.w + c, nv, w[k]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) heavy |= fabsf(w[k][i]) >= 0x1p64f;
+    }
   }
   Ask<T, R> x[K], b[K];
   auto ask = [&](int64_t r) {
@@ -146,39 +181,50 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum = fmaf(v[k][i], v[k][i], sum);
       }
-      // A thread's squares in fp32, the row's in 64 bits: what a row's values share costs them no accuracy.
-      const double root = 1.0 / sqrt(row_sum<NT, double>((double)sum, red) / (double)a.cols + (double)a.eps);
-      const float rstd = (float)root, rest = (float)(root - (double)rstd);
-      if (in && l == 0 && a.rstd) a.rstd[r] = rstd;
+      // A thread's squares in fp32, the row's in 64 bits: what a row's values share costs them no accuracy.  Where fp32
+      // does not hold the squares (values above 2^63, or below 2^-50 with an eps as small) they are added up once more.
+      double total = row_sum<NT, double>((double)sum, red);
+      const bool again = total == __builtin_inf() || (a.eps < 0x1p-100f && total < 0x1p-90);
+      if (__any(again)) {  // (a row that a workgroup shares has all its waves here)
+        double exact = 0.0;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
-        // (s may be x or residual: it is stored behind the row sum, when no thread reads them any more)
-        if (a.s && nv > 0) st_row<T, 8, R>((T*)a.s + r * a.lds + c, nv, v[k]);
-        float y[8];
-        unsigned tie = 0;
+        for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          // v rstd w, with the product's rounding error and rstd's rest put back: rounded once
-          const float p = v[k][i] * w[k][i], e = fmaf(v[k][i], w[k][i], -p);
-          y[i] = i < nv ? fmaf(p, rstd, fmaf(p, rest, e * rstd)) : 0.f;
-          tie |= (__float_as_uint(y[i]) & 0x7ffffu) == 0u;
-        }
-        if (MODE == 1 && tie) {
-          // y that lies half way between two e4m3 values (these have their last 19 bits clear; so have zeros) may
-          // have got there by its own rounding: it moves to the side that the exact value is on
+          for (int i = 0; i < 8; ++i) exact = fma((double)v[k][i], (double)v[k][i], exact);
+        exact = row_sum<NT, double>(exact, red);
+        if (again) total = exact;
+      }
+      const double root = 1.0 / sqrt(total / (double)a.cols + (double)a.eps);
+      // v w may be past what fp32 holds where y is not, and rstd below its normal range: a row's size is taken away first,
+      // by a power of two, 1 at most (1 for a row with infinities, whose root is 0, or NaN).  For 16-bit rows in the
+      // 8-bit form, which wait for their arithmetic, that is a branch of its own, for rows with a mean square of 2^60 and
+      // more, or of 1 with a weight of 2^64 and more (196608 x 256 bf16 75 us, 90 without it; 24571 x 1024 31.3 and 36;
+      // fp32 rows, whose registers it takes, 4096 x 8192 90 and 86).
+      int exponent = (int)(__builtin_bit_cast(unsigned long long, root) >> 52 & 0x7ff) - 1023;
+      if (exponent < -200 || exponent >= (kBranch && !heavy ? -30 : 0)) exponent = 0;
+      const double mant = __builtin_ldexp(root, -exponent);
+      const float rstd = (float)mant, rest = (float)(mant - (double)rstd), up = __builtin_ldexpf(1.f, exponent);
+      if (in && l == 0 && a.rstd) a.rstd[r] = (float)root;
+      // (s may be x or residual: it is stored behind the row sum, when no thread reads them any more)
+      if constexpr (kBranch) {
+        auto row = [&](float up) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float p = v[k][i] * w[k][i], e = fmaf(v[k][i], w[k][i], -p);
-            const float d = fmaf(p, rstd, -y[i]) + fmaf(p, rest, e * rstd);
-            const unsigned u = __float_as_uint(y[i]);
-            if (i < nv && (u & 0x7ffffu) == 0u && (u << 1) != 0u && (u << 1) < 0xff000000u && d != 0.f)
-              y[i] = __uint_as_float((d > 0.f) == (y[i] > 0.f) ? u + 1u : u - 1u);
+          for (int k = 0; k < K; ++k) {
+            const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
+            if (a.s && nv > 0) st_row<T, 8, R>((T*)a.s + r * a.lds + c, nv, v[k]);
+            scale8<true>(v[k], w[k], up, rstd, rest, nv);
           }
-        }
+        };
+        if (__any(exponent != 0)) row(up);
+        else row(1.f);
+      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[k][i] = y[i];
-        if (MODE == 0 && nv > 0) st_row<T, 8, R>((T*)a.y + r * a.ldy + c, nv, v[k]);
+        for (int k = 0; k < K; ++k) {
+          const int c = (k * NT + l) * 8, nv = in ? a.cols - c : 0;
+          if (a.s && nv > 0) st_row<T, 8, R>((T*)a.s + r * a.lds + c, nv, v[k]);
+          scale8<MODE == 1>(v[k], w[k], up, rstd, rest, nv);
+          if (MODE == 0 && nv > 0) st_row<T, 8, R>((T*)a.y + r * a.ldy + c, nv, v[k]);
+        }
       }
     }
     if constexpr (MODE != 0) {

@@ -5,7 +5,7 @@ import torch
 
 from dssm_amd import api
 from tests import seqops_ref as ref
-from tests.test_gpu_seqops import BF, F16, F32, check_blocks, gen, inputs, near, product, rounded
+from tests.test_gpu_seqops import BF, F16, F32, NORM, U, check_blocks, gen, inputs, near, product, rounded
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -79,3 +79,41 @@ def test_product_of_wide_rows(device, M, N, K):
     bias = torch.randn(N, generator=g)
     want, tol = product(a, w, bias, K)
     rounded(api.blocks8_matmul(a, w, bias.to(device)), want, tol)
+
+
+# ---- norm --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("cols", [1, 7, 40, 200, 500, 1000, 2000, 4100, 8000, 16384])
+def test_norm_of_the_largest_and_smallest_rows(device, cols, dtype):
+    """Rows whose squares, and whose products with the weight, are past fp32's range; rows beside them as ever."""
+    g = gen(cols)
+    x = torch.randn(13, cols, generator=g).to(dtype)
+    w = torch.rand(cols, generator=g) + 0.5
+    w[cols // 2] = 1e12
+    dy, ds = torch.randn(13, cols, generator=g).to(dtype), torch.randn(13, cols, generator=g).to(dtype)
+    plain, _, _ = api.rms_norm(x.to(device), w.to(device))
+    plain8, _ = api.rms_norm_blocks8(x.to(device), w.to(device))
+    big = {1: 2.0 ** 60, 3: 2.0 ** 64, 4: 2.0 ** 100, 6: 2.0 ** 120, 9: 2.0 ** 125, 12: 2.0 ** -90}
+    for r, f in big.items():
+        x[r] *= f
+    x[9] = x[9].sign() * 2.0 ** 127  # the largest power of two: the squares' sum is 2^254 times the columns
+    y, s, rstd = api.rms_norm(x.to(device), w.to(device))
+    eps = float(torch.tensor(1e-6))
+    wy, ws, wr = ref.norm(x, w, None, eps)
+    rounded(y, wy, NORM * wy.abs())
+    rounded(rstd, wr[:, 0], NORM * wr[:, 0])
+    y8, _ = api.rms_norm_blocks8(x.to(device), w.to(device))
+    check_blocks(y8, wy, NORM * wy.abs())
+    others = [r for r in range(13) if r not in big]
+    assert torch.equal(y[others], plain[others])
+    assert torch.equal(y8.q.view(torch.uint8)[others], plain8.q.view(torch.uint8)[others])
+    dx, dw = api.rms_norm_grad(dy.to(device), s, w.to(device), rstd, ds.to(device))
+    wx, wdw, mx, mw = ref.norm_grad(dy, ws, w, wr, ds)
+    rounded(dx, wx, 2 * NORM * mx)
+    near(dw, wdw, 53 * U * mw)
+    # an eps as small as the squares of such rows
+    x[12] = (torch.randn(cols, generator=g) * 2.0 ** -74).to(dtype)
+    y, _, rstd = api.rms_norm(x.to(device), w.to(device), None, 2.0 ** -147)
+    wy, _, wr = ref.norm(x, w, None, 2.0 ** -147)
+    rounded(y, wy, NORM * wy.abs())
+    rounded(rstd, wr[:, 0], NORM * wr[:, 0])
