@@ -355,22 +355,25 @@ def _check8(b: Blocks8, what: str) -> int:
 
 
 def rms_norm_blocks8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
-                     eps: float = 1e-6) -> Tuple[Blocks8, torch.Tensor]:
-    """`rms_norm` with its output in 8 bits, for `blocks8_matmul` -> (Blocks8 over the flattened rows, s)."""
+                     eps: float = 1e-6, save: bool = False):
+    """`rms_norm` with its output in 8 bits, for `blocks8_matmul` -> (Blocks8 over the flattened rows, s), with
+    save=True also the rstd [rows] fp32 that `rms_norm_grad` takes (the gradient of the norm without the
+    rounding to 8 bits)."""
     code, weight = _norm_args(x, weight, residual, eps)
     dev = _on_gpu(x, weight, residual)
     cols = x.shape[-1]
     x2, ldx = _rows(x)
     rows = x2.shape[0]
     y = _empty8(rows, cols, dev)
+    rstd = _empty(rows, dtype=torch.float32, device=dev) if save else None
     r2, ldr, s = None, 0, x
     if residual is not None:
         r2, ldr = _rows(residual)
         s = _empty(x.shape, dtype=x.dtype, device=dev)
     if rows:
         _call(dev, "dssm_rms_norm_blocks8", x2.data_ptr(), ldx, _ptr(r2), ldr, weight.data_ptr(), rows, cols, code, float(eps),
-              y.q.data_ptr(), y.scale.data_ptr(), 0 if r2 is None else s.data_ptr(), cols, 0)
-    return y, s
+              y.q.data_ptr(), y.scale.data_ptr(), 0 if r2 is None else s.data_ptr(), cols, _ptr(rstd))
+    return (y, s, rstd) if save else (y, s)
 
 
 def quantize_blocks8(x: torch.Tensor) -> Blocks8:

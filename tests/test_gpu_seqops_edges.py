@@ -117,3 +117,20 @@ def test_norm_of_the_largest_and_smallest_rows(device, cols, dtype):
     wy, _, wr = ref.norm(x, w, None, 2.0 ** -147)
     rounded(y, wy, NORM * wy.abs())
     rounded(rstd, wr[:, 0], NORM * wr[:, 0])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("cols", [5, 96, 300, 1500, 9000])
+def test_norm_to_8_bits_keeps_what_its_gradient_takes(device, cols, dtype):
+    g = gen(cols)
+    x, res, dy = (torch.randn(2, 7, cols, generator=g).to(dtype).to(device) for _ in range(3))
+    w = (torch.rand(cols, generator=g) + 0.5).to(device)
+    for residual in (res, None):
+        _, s, rstd = api.rms_norm(x, w, residual)
+        b, s8 = api.rms_norm_blocks8(x, w, residual)
+        b2, s2, rstd2 = api.rms_norm_blocks8(x, w, residual, save=True)
+        assert torch.equal(s2, s) and torch.equal(s8, s) and torch.equal(rstd2, rstd)
+        assert torch.equal(b2.q.view(torch.uint8), b.q.view(torch.uint8))
+        for p, q in zip(api.rms_norm_grad(dy, s2, w, rstd2), api.rms_norm_grad(dy, s, w, rstd)):
+            assert torch.equal(p, q)
+    assert api.rms_norm_blocks8(x[:0], w, save=True)[2].shape == (0,)
