@@ -134,3 +134,75 @@ def test_norm_to_8_bits_keeps_what_its_gradient_takes(device, cols, dtype):
         for p, q in zip(api.rms_norm_grad(dy, s2, w, rstd2), api.rms_norm_grad(dy, s, w, rstd)):
             assert torch.equal(p, q)
     assert api.rms_norm_blocks8(x[:0], w, save=True)[2].shape == (0,)
+
+
+# ---- embedding ---------------------------------------------------------------------------------------
+# (bits a digit, pairs a thread, sums of the counts): vocabularies from 2^20 words on take three digits, the third pass
+# of which leaves the pairs where the first one did; ids outside the table sort behind all others in every digit
+@pytest.mark.parametrize("n,V,E", [(4097, 1 << 20, 3), (70000, (1 << 20) + 5, 2), (600001, (1 << 21) - 1, 1),
+                                   (2200003, (1 << 20) + 1, 1), (5000, (1 << 27) + 3, 1), (70001, (1 << 28) - 1, 1),
+                                   (300001, (1 << 29) + 7, 1), (4500, (1 << 30) - 1, 1)])
+def test_lookup_grad_of_three_digits(device, n, V, E):
+    g = torch.Generator(device).manual_seed(n)
+    dy = torch.randn(n, E, generator=g, device=device)
+    ids = (torch.rand(n, generator=g, device=device, dtype=torch.float64) ** 6 * V).long().clamp_(0, V - 1)
+    ids[::7] = ids[0]  # a token in all parts of the list
+    ids[3::11] = V - 1 - ids[3::11] // 2  # and large ones
+    ids[5::13], ids[6::17] = -1, V
+    dy[(ids < 0) | (ids >= V)] = float("nan")  # never read
+    got = api.embedding_grad(dy, ids.to(torch.int32) if n % 2 else ids, V, 0.5)
+    ok = (ids >= 0) & (ids < V)
+    words, at = torch.unique(ids[ok], return_inverse=True)
+    want, mag, count = ref.lookup_grad(dy[ok].cpu(), at.cpu(), len(words), 0.5)
+    near(got[words], want, U * (count + 2) * mag)
+    got[words] = 0
+    assert not got.any()  # every other word's row is zero
+
+
+# ---- graphs ------------------------------------------------------------------------------------------
+def test_every_call_in_one_graph(device):
+    """Each call captured, several replays with other inputs and eager work between them, against the eager results."""
+    g = torch.Generator(device).manual_seed(4)
+    R, T, H, E, V = 3, 2400, 64, 130, 700
+    normal = lambda *s: torch.randn(*s, generator=g, device=device)  # noqa: E731
+    ids = torch.randint(0, V, (5000,), generator=g, device=device)
+    few = torch.randint(0, V, (9,), generator=g, device=device, dtype=torch.int32)
+    lens = torch.randint(0, T + 1, (R,), generator=g, device=device)
+    floats = dict(table=normal(V, E), dy=normal(5000, E), gate=normal(R, T, H), cand=normal(R, T, H), dh=normal(R, T, H),
+                  state=normal(R, H), x=normal(300, E), res=normal(300, E), w=normal(E), lin=normal(90, E), bias=normal(90))
+
+    def work(a):
+        out = [api.embedding_lookup(a["table"], ids, 2.0, BF), api.embedding_grad(a["dy"], ids, V),
+               api.embedding_grad(a["dy"][:9], few, V)]
+        h, last, states = api.linear_recurrence(a["gate"], a["cand"], lens, a["state"], True, save=True)
+        out += [h, last, *api.linear_recurrence_grad(a["gate"], a["cand"], states, a["dh"], a["state"], lens, True)]
+        running = a["state"].clone()
+        out += [api.linear_recurrence_step(a["gate"][:, 0], a["cand"][:, 1], running), running]
+        y, s, rstd = api.rms_norm(a["x"], a["w"], a["res"])
+        out += [y, s, rstd, *api.rms_norm_grad(y, s, a["w"], rstd, a["x"])]
+        b, s8, rstd8 = api.rms_norm_blocks8(a["x"], a["w"], a["res"], save=True)
+        lin = api.quantize_blocks8(a["lin"])
+        wide = api.quantize_blocks8(a["dy"].view(-1, 65000))
+        out += [b.q.view(torch.uint8), b.scale.view(torch.uint8), s8, rstd8, lin.q.view(torch.uint8),
+                lin.scale.view(torch.uint8), api.dequantize_blocks8(b, F32), api.dequantize_blocks8(wide, BF)]
+        out += [api.blocks8_matmul(b, lin, a["bias"], F16), api.blocks8_matmul(lin, b)]
+        return out
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(floats)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = work(floats)
+    for k in range(4):
+        for v in floats.values():
+            v.copy_(torch.randn(v.shape, generator=g, device=device))
+        for c in captured:
+            c.zero_()
+        want = [w.clone() for w in work(floats)]
+        graph.replay()
+        eager = work(floats)
+        torch.cuda.synchronize()
+        for i, (a, b, c) in enumerate(zip(captured, want, eager)):
+            assert torch.equal(a, b) and torch.equal(a, c), (k, i)
