@@ -44,6 +44,7 @@ namespace seq {
 namespace {
 
 constexpr int kPiece = DSSM_RECUR_PIECE;
+constexpr int kSegWaves = 8;  // the waves of a workgroup where time is cut into segments (cut_of)
 
 // u = sigmoid(f) and v = 1 - u, neither a difference: e = exp(-|f|) never overflows, and whichever of u and v
 // is small keeps its relative accuracy.  The hardware's 2^x is off by the rounding of its argument, |x| half
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(NW * 64) void k_recur_fwd(RecurArgs a) {
   }
   Piece<T, V, W> in;
   in.ask(g, c, s * a.L + w * kPiece, t.lo, min(t.hi, min(s * a.L + a.L, a.T)));
-  if constexpr (!SUM && NW > 1)
+  if constexpr (!SUM && NW == kSegWaves)
     if (a.S > 1) enter_segment<V, NW>(a, t, s, 1, lds[0], carry);
   const int end = min(s * a.L + a.L, a.T), hi = min(t.hi, end);
   int buf = 0;
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(NW * 64) void k_recur_bwd(RecurArgs a) {
       if (t.in && q0 >= begin && q0 < a.T) st = ldv<float, V>(a.states + (int64_t)(q0 / kPiece) * a.R * a.H + t.ch);
   };
   ask(top + w * kPiece);
-  if constexpr (!SUM && NW > 1)
+  if constexpr (!SUM && NW == kSegWaves)
     if (a.S > 1) enter_segment<V, NW>(a, t, s, -1, lds[0], carry);
   int buf = 0;
   for (int p0 = top; p0 >= begin; p0 -= NW * kPiece, buf ^= 1) {
@@ -535,9 +536,9 @@ Cut cut_of(int64_t R, int T, int H, int dtype) {
   c.NW = 1;
   c.S = 1;
   if (waves < 1024 && pieces > 1) {
-    c.NW = pieces >= 5 ? 8 : 4;
+    c.NW = pieces >= 5 ? kSegWaves : 4;
     const int64_t want = 4096 / (waves * c.NW);
-    if (want >= 2 && pieces > 4 * c.NW) c.S = (int)std::min<int64_t>(want, (pieces + 2 * c.NW - 1) / (2 * c.NW));
+    if (c.NW == kSegWaves && want >= 2 && pieces > 4 * c.NW) c.S = (int)std::min<int64_t>(want, (pieces + 2 * c.NW - 1) / (2 * c.NW));
   }
   const int round = c.NW * kPiece, per = (T + c.S - 1) / c.S;
   c.L = (per + round - 1) / round * round;
@@ -556,11 +557,11 @@ void launch(const RecurArgs& a, const Cut& c, hipStream_t s) {
   auto go = [&](auto nw) {
     constexpr int NW = decltype(nw)::value;
     if constexpr (FWD) {
-      if constexpr (NW > 1)
+      if constexpr (NW == kSegWaves)
         if (c.S > 1) hipLaunchKernelGGL((k_recur_fwd<T, V, NW, true, W>), grid, dim3(NW * 64), 0, s, a);
       hipLaunchKernelGGL((k_recur_fwd<T, V, NW, false, W>), grid, dim3(NW * 64), 0, s, a);
     } else {
-      if constexpr (NW > 1)
+      if constexpr (NW == kSegWaves)
         if (c.S > 1) hipLaunchKernelGGL((k_recur_bwd<T, V, NW, true, W>), grid, dim3(NW * 64), 0, s, a);
       hipLaunchKernelGGL((k_recur_bwd<T, V, NW, false, W>), grid, dim3(NW * 64), 0, s, a);
     }

@@ -84,3 +84,11 @@ def test_a_steps_rows_that_overlap_are_refused():
     assert step(P, 4, P, 4, F32, P, 0, P, 4, 2, 4, 0) == -1
     assert step(P, 4, P, 4, F32, P, 4, P, -3, 2, 4, 0) == -1
     assert b"overlap" in _lib.load().dssm_last_error()
+
+
+def test_no_recurrence_kernel_is_built_that_no_cut_takes():
+    """Segments of time are summed by eight waves or not at all, so no other kernel for it is in the library."""
+    import re
+
+    names = re.findall(rb"k_recur_[fb]wdI[^_]*?Li\dELi(\d)ELb([01])E", open(_lib.LIB_PATH, "rb").read())
+    assert {(int(nw), int(sums)) for nw, sums in names} == {(1, 0), (4, 0), (8, 0), (8, 1)}
