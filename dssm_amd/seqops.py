@@ -14,7 +14,8 @@ GRU tower of dssm_amd/rnn.py (reference dssm_rnn.py:100-217).
 Each call is one C-ABI entry of include/dssm.h on the current stream of its tensors' device; gradients are
 calls of their own (nothing records a graph).  Tensors are float32, bfloat16 or float16 as said; sums,
 statistics and states are fp32.  All results are new tensors, except where a call says "in place".  Every call
-can be captured into a graph.  Wrong types and shapes raise TypeError / ValueError before anything runs.
+can be captured into a graph.  Wrong types and shapes raise TypeError / ValueError before anything runs.  Autograd does
+not see these calls: a tensor that requires a gradient gets none from them, only from the gradients' own calls.
 """
 from __future__ import annotations
 
@@ -28,6 +29,7 @@ _CODE = {torch.float32: _lib.DSSM_F32, torch.bfloat16: _lib.DSSM_BF16, torch.flo
 BLOCK = 128          # columns that share a scale
 MAX_NORM_COLS = 16384
 MAX_BLOCKS8_COLS = 1 << 22
+MAX_ROWS = 2 ** 31 - 1
 # what rounds to a positive finite float32 lies between these
 _EPS_LOW, _EPS_HIGH = 2.0 ** -150, 2.0 ** 128 - 2.0 ** 103
 _PIECE = 8           # include/dssm.h DSSM_RECUR_PIECE
@@ -91,6 +93,11 @@ def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return x, (s0 if n > 1 else cols)
 
 
+def _row_count(x: torch.Tensor, cols: int) -> None:
+    if x.numel() > MAX_ROWS * cols:
+        raise ValueError(f"at most {MAX_ROWS} rows")
+
+
 def _vector(v: Optional[torch.Tensor], n: int, what: str) -> Optional[torch.Tensor]:
     if v is None:
         return None
@@ -110,7 +117,8 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
                      dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """scale * table[ids]: table [V x E], ids of any shape, int32 or int64 -> [*ids.shape, E] in `dtype`
     (default: the table's).  The product is formed in fp32 and rounded once.  An id outside [0, V) reads
-    nothing and gives a row of zeros (a padding id, say)."""
+    nothing and gives a row of zeros (a padding id, say).  More ids than one launch takes (2^28 - 16 of more than
+    256 columns, more of fewer) raise DssmError."""
     if table.dim() != 2 or 0 in table.shape:
         raise ValueError("table must be [V x E]")
     if table.shape[1] > 1 << 30:
@@ -280,6 +288,7 @@ def _norm_args(x, weight, residual, eps):
     code = _code(x.dtype, "x")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_NORM_COLS:
         raise ValueError(f"x must have 1 to {MAX_NORM_COLS} columns")
+    _row_count(x, x.shape[-1])
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("residual must have x's shape and type")
     if not _EPS_LOW < eps < _EPS_HIGH:
@@ -318,6 +327,7 @@ def rms_norm_grad(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor, rstd:
     if dy.dim() < 1 or not 1 <= dy.shape[-1] <= MAX_NORM_COLS:
         raise ValueError(f"dy must have 1 to {MAX_NORM_COLS} columns")
     cols = dy.shape[-1]
+    _row_count(dy, cols)
     weight = _vector(weight, cols, "weight")
     dy2, lddy = _rows(dy)
     rows = dy2.shape[0]
@@ -383,6 +393,7 @@ def quantize_blocks8(x: torch.Tensor) -> Blocks8:
     code = _code(x.dtype, "x")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_BLOCKS8_COLS:
         raise ValueError(f"x must have 1 to {MAX_BLOCKS8_COLS} columns")
+    _row_count(x, x.shape[-1])
     dev = _on_gpu(x)
     x2, ld = _rows(x)
     b = _empty8(x2.shape[0], x.shape[-1], dev)
@@ -399,6 +410,8 @@ def dequantize_blocks8(b: Blocks8, dtype: torch.dtype = torch.float32) -> torch.
     rows = _check8(b, "b")
     if b.cols > MAX_BLOCKS8_COLS:
         raise ValueError(f"b must have 1 to {MAX_BLOCKS8_COLS} columns")
+    if rows > MAX_ROWS or rows * -(-b.cols // 8) > 2 ** 32 - 2 ** 8:
+        raise ValueError(f"at most {MAX_ROWS} rows and 2^32 - 256 groups of eight values")
     dev = _on_gpu(b.q, b.scale)
     out = _empty(rows, b.cols, dtype=dtype, device=dev)
     if rows:

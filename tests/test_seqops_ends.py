@@ -92,3 +92,14 @@ def test_no_recurrence_kernel_is_built_that_no_cut_takes():
 
     names = re.findall(rb"k_recur_[fb]wdI[^_]*?Li\dELi(\d)ELb([01])E", open(_lib.LIB_PATH, "rb").read())
     assert {(int(nw), int(sums)) for nw, sums in names} == {(1, 0), (4, 0), (8, 0), (8, 1)}
+
+
+def test_more_rows_than_a_call_takes_are_a_value_error():
+    """As the module says of shapes that do not fit, before anything runs."""
+    tall, w = Z(1, 1).expand(1 << 31, 1), Z(1)
+    for call in (lambda: api.rms_norm(tall, w), lambda: api.rms_norm_blocks8(tall, w), lambda: api.quantize_blocks8(tall),
+                 lambda: api.rms_norm_grad(tall, tall, w, Z(1).expand(1 << 31))):
+        with pytest.raises(ValueError, match="rows"):
+            call()
+    with pytest.raises(ValueError, match="GPU"):
+        api.quantize_blocks8(Z(1, 1).expand((1 << 31) - 1, 1))
