@@ -206,3 +206,14 @@ def test_every_call_in_one_graph(device):
         torch.cuda.synchronize()
         for i, (a, b, c) in enumerate(zip(captured, want, eager)):
             assert torch.equal(a, b) and torch.equal(a, c), (k, i)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 20, 700), (300, 260, 700), (64, 1000, 1100), (2100, 2100, 260)])
+def test_product_of_the_furthest_scales(device, M, N, K):
+    """Scales at both ends of their range: of rows in fp32's subnormals, of the largest, and results near both ends."""
+    g = gen(M)
+    for ex, ey in ((-136, 120), (120, -136), (-120, -20), (100, 20), (-60, -60)):
+        x, y = torch.randn(M, K, generator=g), torch.randn(N, K, generator=g) * 2.0 ** ey
+        a, w = (api.quantize_blocks8(t.to(device)) for t in (x * 2.0 ** (ex // 2) * 2.0 ** (ex - ex // 2), y))
+        want, tol = product(a, w, None, K)
+        rounded(api.blocks8_matmul(a, w), want, tol)
