@@ -6,8 +6,9 @@
 // table would add a hot token's rows in any order and one after the other; here the positions are first
 // sorted by token (stable, so a token's positions stay in order), and the sorted list is cut into equal
 // spans whatever the tokens: a span sums the runs of equal tokens it holds in fp32, stores the runs that
-// lie whole inside it, and leaves the (at most two) cut ones as partial rows, which the last launch joins
-// in span order.  The result does not depend on timing, and a token that fills half of the list is
+// lie whole inside it, and leaves the (at most two) cut ones as partial rows, which the last launch joins.  Eight
+// positions are added in their order; their sums, and spans', in a fixed one (one after the other, or by doubling where
+// there are many).  The result does not depend on timing, and a token that fills half of the list is
 // spread over as many workgroups as any other half.
 //
 // The sort is a least-significant-digit radix sort of (token, position) pairs, digits of at most 10 bits;

@@ -81,9 +81,10 @@ __device__ __forceinline__ void store4(const Gemm8Args& g, int m, int n, f32x4 v
 // of the matrix units ahead); 64 x 64 and 32 x 32, which run where there are few tiles and the memory's latency is
 // all there is to a block, take 4.
 //
-// Measured, 8192 x 4096 x 8192: 226 us, 2.4 PFLOP/s, 93 % of the library's rate for one scale a tensor (2.56); the
-// matrix units are busy 62 % of the time at 1.85 GHz, to which their power brings the clock down.  Without the loads
-// the same loop takes 184 us, always from the same two blocks 217.  8192 x 8192 x 4096: 2.3 PFLOP/s.
+// Measured, 8192 x 4096 x 8192: 227 to 233 us a pass among others (224 to 251 under a trace), 2.4 PFLOP/s, 92 to 94 %
+// of the library's rate for one scale a tensor (2.56); the matrix units are busy 62 % of the time at 1.85 GHz, to
+// which their power brings the clock down.  Without the loads the same loop takes 184 us, always from the same two
+// blocks 217.  8192 x 8192 x 4096: 2.3 PFLOP/s.
 //
 // A row's 128 bytes are eight 16-byte pieces; piece p of row r lies at p ^ (r >> 1 & 7).  A 16-byte read serves
 // sixteen lanes a cycle: lanes 0-3, 12-15, 20-23 and 24-27 of a half wave, then the others (found with the
@@ -410,7 +411,7 @@ int run_gemm8(const Gemm8Args& g, hipStream_t s) {
   if (tiles(64) > 0x7fffffff) return dssm::report_error(DSSM_E_UNSUPPORTED, "blocks8_matmul: too many outputs");
   const int tile = tile_of(tiles(64), tiles(128), tiles(256));
   // Rows against rows where that takes a workgroup a compute unit at most: the waves of a workgroup share K (7 x 4096 x
-  // 4096: 5.9 us against 8.5 in 32 x 32 tiles, 32 x 256 x 8192 10.0 against 11.6, 100 x 300 x 200 2.9 against 4.3);
+  // 4096: 5.9 us (6.1 to 6.8 traced) against 8.5 in 32 x 32 tiles, 32 x 256 x 8192 10.0 against 11.6, 100 x 300 x 200 2.9 against 4.3);
   // 32 rows at a time for 17 to 32 of them (32 x 4096 x 4096: 8.8 us, 10.7 sixteen at a time, 9.1 in tiles).  With more
   // workgroups, each of which reads its rows of a again, tiles are faster (32 x 8192 x 1024 5.6 us against 8.4, 16 x
   // 12288 x 4096 12.3 against 14.6).

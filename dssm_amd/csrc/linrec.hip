@@ -25,8 +25,8 @@
 // gates and sums are fp32 throughout.
 //
 // Measured: 6144 rows x 32 steps x 128 channels bf16, ragged, 29 us forward and 43 backward (3.9 and 4.3 TB/s of
-// the bytes that ragged rows leave); 2 x 65537 x 512 bf16 68 + 74 us, 4 x 16411 x 256 fp32 ragged 32 + 30 forward
-// and 28 + 53 backward (the replaying launches 5.0 to 5.5 TB/s, memory; the summing ones read at 4 TB/s).  A
+// the bytes that ragged rows leave); 2 x 65537 x 512 bf16 68 + 74 us, 4 x 16411 x 256 fp32 ragged 32 + 31 forward
+// and 29 + 54 backward (the replaying launches 5.0 to 5.5 TB/s, memory; the summing ones read at 4 TB/s).  A
 // piece of 16 steps keeps twice the registers and half the waves (backward 51 us, 84 + 101 for the long rows).
 // (One launch whose segments wait for each other's sums would read the inputs once; it is not taken: a wait between
 // running workgroups for a third of the time of few, very long rows.)
@@ -47,9 +47,9 @@ constexpr int kPiece = DSSM_RECUR_PIECE;
 constexpr int kSegWaves = 8;  // the waves of a workgroup where time is cut into segments (cut_of)
 
 // u = sigmoid(f) and v = 1 - u, neither a difference: e = exp(-|f|) never overflows, and whichever of u and v
-// is small keeps its relative accuracy.  The hardware's 2^x is off by the rounding of its argument, |x| half
-// units: for fp32 gates that rounding and log2 e's own are put back, for gates that were rounded to 16 bits
-// (whose own half step moves e by |x| 2^-12 and more) they are not.
+// is small keeps its relative accuracy down to 2^-126 (|f| = 87.3), below which it is 0.  The hardware's 2^x is off
+// by the rounding of its argument, |x| half units: for fp32 gates that rounding and log2 e's own are put back, for
+// gates that were rounded to 16 bits (whose own half step moves e by |x| 2^-12 and more) they are not.
 template <typename T>
 __device__ __forceinline__ void gate_uv(float f, float& u, float& v) {
   const float kL = 1.44269502f, kLlo = 1.92596303e-8f;

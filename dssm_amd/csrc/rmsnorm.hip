@@ -12,9 +12,9 @@
 // block of 128 columns, so a block's scale is four DPP steps away.  A workgroup stays for many rows, its weights in
 // registers, with the next row's loads behind the current one's arithmetic.
 //
-// Measured: 196608 x 256 bf16 with a residual 68 us forward, 83 + 5 backward (403 MB each way: 5.9 and 4.6 TB/s, the
+// Measured: 196608 x 256 bf16 with a residual 68 us forward, 82 + 5 backward (403 MB each way: 5.9 and 4.6 TB/s, the
 // forward's inputs in part still cached; one workgroup for every four rows took 117 and 119); 24571 x 1024 to the
-// 8-bit form 35 us (5.0 TB/s), its values back in bf16 14 us (5.4 TB/s).
+// 8-bit form 34 us (5.1 TB/s), its values back in bf16 13 us (5.8 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -251,7 +251,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_bwd(NormArgs a) {
   constexpr int kRows = NT < 256 ? 256 / NT : 1;
   __shared__ float red[16];
   // the next row's loads in flight behind this one's arithmetic, but where 1024 threads hold 16 columns each: their
-  // 128 registers take no second row (16384 x 4096 bf16 110 us; 191 with both, which spills)
+  // 128 registers take no second row (16384 x 4096 bf16 110 us; 191 with both, which spills).  (More than 8192 columns
+  // that are no multiple of 8 spill 8 registers all the same, fp32 14.)
   constexpr bool kAhead = NT * K < 2048;
   __shared__ float slot[kRows > 1 ? kRows : 1][kRows > 1 ? NT * 8 + 4 : 1];
   const int l = threadIdx.x % NT, g = threadIdx.x / NT;

@@ -12,10 +12,11 @@ GRU tower of dssm_amd/rnn.py (reference dssm_rnn.py:100-217).
   scale for each 128 columns (`Blocks8`), and their product with a layer's weights.
 
 Each call is one C-ABI entry of include/dssm.h on the current stream of its tensors' device; gradients are
-calls of their own (nothing records a graph).  Tensors are float32, bfloat16 or float16 as said; sums,
-statistics and states are fp32.  All results are new tensors, except where a call says "in place".  Every call
-can be captured into a graph.  Wrong types and shapes raise TypeError / ValueError before anything runs.  Autograd does
-not see these calls: a tensor that requires a gradient gets none from them, only from the gradients' own calls.
+calls of their own.  Autograd does not see any of them: a tensor that requires a gradient gets none from these
+calls, only from the gradients' own.  Tensors are float32, bfloat16 or float16 as said; sums, statistics and
+states are fp32 (a row's sum of squares 64 bits).  All results are new tensors, except where a call says "in
+place".  Every call can be captured into a graph.  Wrong types and shapes raise TypeError / ValueError before
+anything runs.
 """
 from __future__ import annotations
 
@@ -204,7 +205,8 @@ def linear_recurrence(gate: torch.Tensor, cand: torch.Tensor, lens: Optional[tor
                       h0: Optional[torch.Tensor] = None, reverse: bool = False, save: bool = False):
     """h_t = u_t h_{t-1} + (1 - u_t) cand_t, u = sigmoid(gate), over gate, cand [R x T x H] of any row and time
     strides (both halves of one projection, or time-major storage transposed) -> (h [R x T x H] in their
-    type, last [R x H] fp32), with save=True also the states that `linear_recurrence_grad` takes.
+    type, last [R x H] fp32), with save=True also the states that `linear_recurrence_grad` takes.  u and 1 - u below
+    2^-126 (gates past 87.3 either way) count as 0.
 
     lens [R]: a row's steps, clamped to [0, T]; the steps behind them are not read, h is zero there and
     `last` is the state at the row's end (h0 for an empty row), as tf.nn.dynamic_rnn has it.  h0 [R x H]

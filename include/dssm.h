@@ -694,16 +694,16 @@ int dssm_rnn_adam_ex(float* p, const float* g, float* m, float* v, int64_t n_spa
  * The pieces of a gated recurrent tower over token ids beside the GRU tower (dssm_rnn.py:100-217): its
  * lookup, a recurrence whose gates do not look at the state (so that time can be cut), the norm between
  * layers, and the 8-bit product.  Storage types dtype / out_dtype: DSSM_F32, DSSM_BF16, DSSM_F16; sums,
- * statistics and states are fp32.  Leading dimensions and strides are in elements, rows may start at any
- * element.  Sizes of zero rows do nothing, and pointers to such rows may be NULL (gradients that are sums over rows are
- * zeros).  Outputs must not overlap inputs unless a call says so. */
+ * statistics and states are fp32 (a row's sum of squares 64 bits).  Leading dimensions and strides are in
+ * elements, rows may start at any element.  Sizes of zero rows do nothing, and pointers to such rows may be NULL
+ * (gradients that are sums over rows are zeros).  Outputs must not overlap inputs unless a call says so. */
 
 /* tf.nn.embedding_lookup(table, ids) * scale (dssm_rnn.py:113-118): out [n x E] from table [V x E] (row
  * stride ldt).  ids: int32, or int64 with ids64; an id outside [0, V) gives a row of zeros.  E <= 2^30. */
 int dssm_embedding_lookup(const void* table, int dtype, int64_t ldt, int64_t V, int E, const void* ids, int ids64,
                           int64_t n, float scale, void* out, int out_dtype, void* stream);
 /* Its gradient: dtable [V x E] fp32 (16-byte aligned, every row written) = scale * the rows of dy [n x E]
- * summed by token, in the order of their positions (the result does not depend on timing); ids outside
+ * summed by token, in a fixed order (the result does not depend on timing); ids outside
  * [0, V) are left out.  n < 2^31 - 4096, V < 2^30, E <= 2^20.  ws: dssm_embedding_grad_ws_bytes() bytes,
  * 16-byte aligned, of any content (0: a size is out of range). */
 size_t dssm_embedding_grad_ws_bytes(int64_t n, int64_t V, int E, int dtype);
@@ -711,12 +711,12 @@ int dssm_embedding_grad(const void* dy, int dtype, int64_t lddy, const void* ids
                         float scale, float* dtable, void* ws, size_t ws_bytes, void* stream);
 
 /* Gated linear recurrence over [R x T x H]: u = sigmoid(gate), h_t = u_t h_{t-1} + (1 - u_t) cand_t (the
- * GRUCell's convention without its state-dependent gates).  Row and time strides of gate, cand and h are
- * free (both halves of one projection, time-major storage).  lens [R] (NULL: T; clamped to [0, T]): steps
- * at or past it are not read, emit zero and carry the state.  reverse: from the row's last step to its
- * first.  h0 [R x H] fp32 or NULL (zeros); last [R x H] fp32: the state after the walk.  states (NULL for
- * inference): ceil(T / DSSM_RECUR_PIECE) x R x H floats, the state in front of every DSSM_RECUR_PIECE steps of
- * the walk, read by the backward.  ws: dssm_linear_recurrence_ws_bytes() bytes of any content (0: none
+ * GRUCell's convention without its state-dependent gates); u and 1 - u below 2^-126 count as 0.  Row and time
+ * strides of gate, cand and h are free (both halves of one projection, time-major storage).  lens [R] (NULL: T;
+ * clamped to [0, T]): steps at or past it are not read, emit zero and carry the state.  reverse: from the row's
+ * last step to its first.  h0 [R x H] fp32 or NULL (zeros); last [R x H] fp32: the state after the walk.  states
+ * (NULL for inference): ceil(T / DSSM_RECUR_PIECE) x R x H floats, the state in front of every DSSM_RECUR_PIECE
+ * steps of the walk, read by the backward.  ws: dssm_linear_recurrence_ws_bytes() bytes of any content (0: none
  * is needed, ws may be NULL); forward and backward need the same.  1 <= T <= 2^28, 1 <= H <= 2^20, R * H <= 2^31. */
 #define DSSM_RECUR_PIECE 8
 size_t dssm_linear_recurrence_ws_bytes(int64_t R, int T, int H, int dtype);
